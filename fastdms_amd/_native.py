@@ -69,6 +69,10 @@ SIGNATURES: dict[str, str] = {
     "fdms_fused_decode_attention_paged": "pllpllpllpllppllpllfffipplpllipllpllppiiiiiifppppfp",
     "fdms_fused_decode_attention_planned": "pllpllpllpllpppllfffipplpllppiiiiifppppfp",
     "fdms_fp8_gemm": "plpplpppliiip",
+    "fdms_block_tables": "ppiplipipiippppppp",
+    "fdms_store_block_kvcache": "ppillllppillllpplpiiiiip",
+    "fdms_gather_block_kvcache": "ppillllpplpiiiiippillllp",
+    "fdms_block_attention": "pillippillllpplplipppllpiiiiiiiiifp",
 }
 
 _CT = {"p": _P, "i": _I, "l": _L, "f": _F}

@@ -36,6 +36,7 @@ CFLAGS = [
 # default there) every block copies them out and back.
 FILE_FLAGS = {
     "prefill_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "block_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],  # the same softmax between two products
     # The decode attention kernels take the arguments their first loads need
     # first (the plan of the planned launch, the live counts, append rows and
     # positions of the others); preloading them into SGPRs at

@@ -1,0 +1,312 @@
+"""Dense 8-bit block KV cache: its tables, store, read-back and attention.
+
+The cache that keeps every token, beside the compact one that DMS evicts from
+(the reference's dense paged path, attention.py:17-37, 94-100, keeps bf16 rows
+and calls flash-attn).  Blocks of ``block_size`` tokens (a power of two,
+16 .. 256) hold each kv head's rows in 8 bits with one scale per (block, head)
+for K and one for V:
+
+    k_cache [blocks, heads, block_size, D]          int8 or float8_e4m3fn
+    v_cache [blocks, heads, block_size / 16, D, 16] V in transposed 16-token tiles
+    k_scale, v_scale [blocks, heads]                fp32
+
+A code stands for code * scale; the store's scales are powers of two.  A step
+runs ``prepare_block_tables`` once, then per layer ``store_block_kvcache`` and
+``block_attention``; ``gather_block_kvcache`` reads rows back dense, e.g. to
+pack a prompt into the compact layout.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from .. import _native as nat
+
+TILE = 16            # tokens per transposed V tile
+MAX_SEQS = 4096      # sequences per prepare_block_tables call
+BLOCK_SIZES = (16, 32, 64, 128, 256)
+CACHE_DTYPES = (torch.int8, torch.float8_e4m3fn)
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_INT_MAX = 2 ** 31 - 1
+
+# bits of BlockTables.status
+STATUS_NO_BLOCKS, STATUS_TABLE_WIDTH, STATUS_NUM_TOKENS, STATUS_INVALID = 1, 2, 4, 8
+
+
+class BlockTables(NamedTuple):
+    """A step's metadata, on the device (prepare_block_tables)."""
+    slot_mapping: torch.Tensor   # int32 [num_tokens], -1 past the step's last token
+    positions: torch.Tensor      # int64 [num_tokens], 0 past the step's last token
+    cu_seqlens: torch.Tensor     # int32 [seqs + 1]
+    context_lens: torch.Tensor   # int32 [seqs], cached + new
+    free_count: torch.Tensor     # int32 [1], what is left of the stack
+    status: torch.Tensor         # int32 [1], 0 or STATUS_* bits
+
+
+def allocate_block_kvcache(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int,
+                           dtype: torch.dtype = torch.int8, device="cuda"):
+    """(k_cache, v_cache, k_scale, v_scale) of ``num_blocks`` blocks; the codes
+    are not initialised."""
+    if dtype not in CACHE_DTYPES:
+        raise ValueError(f"a block KV cache holds int8 or float8_e4m3fn, got {dtype}")
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"the block KV cache supports head_dim 64 or 128, got {head_dim}")
+    if num_blocks < 1 or num_kv_heads < 1 or num_blocks * block_size > _INT_MAX:
+        raise ValueError("a block KV cache needs at least one block and head and fewer than 2^31 slots")
+    k = torch.empty((num_blocks, num_kv_heads, block_size, head_dim), device=device, dtype=dtype)
+    v = torch.empty((num_blocks, num_kv_heads, block_size // TILE, head_dim, TILE), device=device, dtype=dtype)
+    return (k, v, torch.zeros((num_blocks, num_kv_heads), device=device),
+            torch.zeros((num_blocks, num_kv_heads), device=device))
+
+
+def _check_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
+    """(blocks, heads, block size, head_dim) of a well-formed cache."""
+    if k_cache.dtype not in CACHE_DTYPES or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"a block KV cache holds int8 or float8_e4m3fn, got {k_cache.dtype} / {v_cache.dtype}")
+    if k_cache.ndim != 4:
+        raise ValueError(f"expected k_cache [blocks, heads, block_size, head_dim], got {tuple(k_cache.shape)}")
+    nb, h, bs, d = k_cache.shape
+    if bs not in BLOCK_SIZES or d not in (64, 128):
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES} and head_dim 64 or 128, got {bs} and {d}")
+    if v_cache.shape != (nb, h, bs // TILE, d, TILE):
+        raise ValueError(f"expected v_cache {(nb, h, bs // TILE, d, TILE)}, got {tuple(v_cache.shape)}")
+    if nb < 1 or nb * bs > _INT_MAX:
+        raise ValueError("a block KV cache needs at least one block and fewer than 2^31 slots")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or ks[2] != d or vs[4] != 1 or vs[3] != TILE or (bs > TILE and vs[2] != TILE * d):
+        raise ValueError("a head's part of a block must be contiguous in k_cache and v_cache")
+    if (ks[0] | ks[1] | vs[0] | vs[1] | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("k_cache and v_cache blocks must be 16-byte aligned")
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or s.shape != (nb, h) or (h > 1 and s.stride(1) != 1):
+            raise ValueError(f"expected fp32 scales [{nb}, {h}] with contiguous heads")
+    if nb > 1 and k_scale.stride(0) != v_scale.stride(0):
+        raise ValueError("k_scale and v_scale must have the same block stride")
+    return nb, h, bs, d
+
+
+def _on_device(what: str, *tensors) -> torch.device:
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev or dev.type != "cuda":
+            raise RuntimeError(f"{what} requires its tensors on one GPU (HIP device); got {t.device} and {dev}")
+    return dev
+
+
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """nat.call on the tensors' device, on its current stream."""
+    if dev.index == torch.cuda.current_device():
+        nat.call(name, *args, nat.stream())
+    else:
+        with torch.cuda.device(dev):
+            nat.call(name, *args, nat.stream())
+
+
+def _int32(what: str, t: torch.Tensor, shape: tuple) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 {list(shape)} tensor, got {t.dtype} {list(t.shape)}")
+
+
+def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
+                         free_blocks: torch.Tensor, free_count: torch.Tensor, *, block_size: int, num_tokens: int,
+                         out: BlockTables | None = None) -> BlockTables:
+    """Block tables and slot map of a step, on the device from its lengths.
+
+    Sequence b holds ``cached_lens[b]`` tokens in the first
+    ``ceil(cached / block_size)`` entries of ``block_tables[b]`` and gets
+    ``new_lens[b]`` (0 or more) in this step.  The blocks it lacks are popped
+    from the stack ``free_blocks[: free_count]``, top first, in the order of
+    the sequences, and written into its table row.  Token t of the step,
+    sequence after sequence, gets its position and its slot
+    ``table[position // block_size] * block_size + position % block_size``;
+    ``num_tokens`` is the length of those outputs and may exceed the step's
+    tokens (a padded batch).  Nothing is read back: the host passes sizes only.
+
+    When the stack, a table row or ``num_tokens`` is too short, or a length or
+    the count is invalid, ``status`` says so (STATUS_* bits) and nothing is
+    popped: the tables stay, every slot is -1, cu_seqlens is 0 and context_lens
+    the cached lengths.  ``free_count`` is not changed in place, so a step can
+    be prepared again; ``out`` takes an earlier call's tensors (captured steps),
+    whose free_count must be another tensor than the argument."""
+    n = cached_lens.numel()
+    if not 1 <= n <= MAX_SEQS:
+        raise ValueError(f"prepare_block_tables takes 1 to {MAX_SEQS} sequences, got {n}")
+    _int32("cached_lens", cached_lens, (n,))
+    _int32("new_lens", new_lens, (n,))
+    _int32("free_blocks", free_blocks, (free_blocks.numel(),))
+    _int32("free_count", free_count, (1,))
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != n:
+        raise ValueError(f"block_tables must be int32 [{n}, blocks], got {block_tables.dtype} "
+                         f"{tuple(block_tables.shape)}")
+    width = block_tables.shape[1]
+    if width > 1 and block_tables.stride(1) != 1 or n > 1 and block_tables.stride(0) < width:
+        raise ValueError("block_tables needs rows of its own with contiguous entries")
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    if not 0 <= num_tokens <= _INT_MAX:
+        raise ValueError(f"num_tokens must be between 0 and {_INT_MAX}, got {num_tokens}")
+    dev = _on_device("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count)
+    if out is None:
+        slots, cu, ctx, count, status = torch.empty(num_tokens + 2 * n + 3, device=dev, dtype=torch.int32).split(
+            (num_tokens, n + 1, n, 1, 1))
+        out = BlockTables(slots, torch.empty(num_tokens, device=dev, dtype=torch.int64), cu, ctx, count, status)
+    else:
+        for what, size in (("slot_mapping", num_tokens), ("cu_seqlens", n + 1), ("context_lens", n),
+                           ("free_count", 1), ("status", 1)):
+            _int32(f"out.{what}", getattr(out, what), (size,))
+        if out.positions.dtype != torch.int64 or out.positions.shape != (num_tokens,) or \
+                not out.positions.is_contiguous():
+            raise ValueError(f"out.positions must be a contiguous int64 [{num_tokens}] tensor")
+        _on_device("prepare_block_tables", cached_lens, *out)
+        if out.free_count.data_ptr() == free_count.data_ptr():
+            raise ValueError("out.free_count must be another tensor than free_count")
+    _launch(dev, "fdms_block_tables", cached_lens.data_ptr(), new_lens.data_ptr(), n, block_tables.data_ptr(),
+            block_tables.stride(0), width, free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(),
+            block_size, num_tokens, out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.cu_seqlens.data_ptr(),
+            out.context_lens.data_ptr(), out.free_count.data_ptr(), out.status.data_ptr())
+    return out
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [rows, heads, D] with a contiguous head_dim and 16-byte aligned rows: itself, or a copy."""
+    size = x.element_size()
+    if x.stride(2) == 1 and not (x.stride(0) * size | x.stride(1) * size | x.data_ptr()) % 16:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def store_block_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Store rows key / value [T, heads, D] (fp32, fp16 or bf16) at their slots.
+
+    ``slot_mapping`` int32 [T] as prepare_block_tables writes it: the rows a
+    call brings to one block are neighbours with consecutive slots and follow
+    the rows that the block holds already (a call whose rows reach one block in
+    several runs leaves that block's contents undefined).  A slot that is
+    negative or past the cache is skipped.
+
+    Per (block, head) the scale is the least power of two s with
+    ``max |x| <= 127 s`` (int8) or ``448 s`` (e4m3fn) over the new rows, at
+    least 2^-126, and no less than the block's scale if it held rows before;
+    codes are x / s rounded to nearest even.  When new rows raise the scale,
+    the earlier rows' codes are rounded again to it.  Infinities saturate
+    (counting as the largest fp32 value for the scale) and NaN is stored as 0:
+    a cached row never poisons another sequence position's attention."""
+    nb, h, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    if key.ndim != 3 or key.shape != value.shape or key.shape[1:] != (h, d):
+        raise ValueError(f"expected key and value [tokens, {h}, {d}], got {tuple(key.shape)} and "
+                         f"{tuple(value.shape)}")
+    if key.dtype not in _FLOATS or value.dtype != key.dtype:
+        raise ValueError(f"key and value must be fp32, fp16 or bf16 alike, got {key.dtype} and {value.dtype}")
+    t = key.shape[0]
+    _int32("slot_mapping", slot_mapping, (t,))
+    dev = _on_device("store_block_kvcache", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    if t == 0:
+        return
+    key, value = _aligned_rows(key), _aligned_rows(value)
+    _launch(dev, "fdms_store_block_kvcache", key.data_ptr(), value.data_ptr(), nat.dtype_code(key.dtype),
+            key.stride(0), key.stride(1), value.stride(0), value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
+            int(k_cache.dtype != torch.int8), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
+            v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), slot_mapping.data_ptr(), t,
+            nb, bs, h, d)
+
+
+def gather_block_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                         slot_mapping: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """Dense (K, V) [T, heads, D] of the rows at ``slot_mapping`` int32 [T]:
+    code * scale, exact in bf16 and fp32 for the store's scales.  Any slots in
+    any order; one that is negative or past the cache gives a row of zeros."""
+    nb, h, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    if dtype not in _FLOATS:
+        raise ValueError(f"gather_block_kvcache returns fp32, fp16 or bf16, not {dtype}")
+    t = slot_mapping.numel()
+    _int32("slot_mapping", slot_mapping, (t,))
+    dev = _on_device("gather_block_kvcache", k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    k = torch.empty((t, h, d), device=dev, dtype=dtype)
+    v = torch.empty((t, h, d), device=dev, dtype=dtype)
+    if t:
+        _launch(dev, "fdms_gather_block_kvcache", k_cache.data_ptr(), v_cache.data_ptr(),
+                int(k_cache.dtype != torch.int8), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
+                v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0),
+                slot_mapping.data_ptr(), t, nb, bs, h, d, k.data_ptr(), v.data_ptr(), nat.dtype_code(dtype),
+                k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    return k, v
+
+
+def block_attention_plan(pairs: int, group: int, max_seqlen: int, max_context: int) -> tuple[int, int, int]:
+    """(query rows per tile, tiles, splits of the keys) of a block_attention
+    launch over ``pairs`` (sequence, kv head) pairs: tiles of 16 rows, or 32
+    when a sequence has more; splits to reach about four workgroups per CU,
+    each of at least 256 keys of the longest context."""
+    max_rows = max_seqlen * group
+    rows = 16 if max_rows <= 16 else 32
+    tiles = -(-max_rows // rows)
+    splits = min(-(-1024 // (pairs * tiles)), -(-max_context // 256), 256)
+    return rows, tiles, max(1, splits)
+
+
+def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, *,
+                    cu_seqlens: torch.Tensor | None = None, max_seqlen: int = 1, max_context: int | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention of q [T, q heads, D] (bf16 or fp16) over the cache.
+
+    Sequence b's keys are the ``context_lens[b]`` rows its ``block_tables``
+    row leads to and its queries rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1``
+    of q, the last of its keys (bottom-right causal alignment, as
+    ``prefill_attention``); without ``cu_seqlens`` row b is sequence b's one
+    query.  ``max_seqlen`` bounds a sequence's queries and ``max_context`` the
+    contexts (default: what a table row can hold); both are host numbers that
+    shape the launch.  A query that sees no key gets zeros, rows past
+    ``cu_seqlens[-1]`` of ``out`` are left as they are, and keys of a block
+    that is not in the cache are left out.  Scales must not be negative.
+    Default ``scale``: D ** -0.5."""
+    nb, h, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    if q.ndim != 3 or q.shape[2] != d or q.shape[1] % h or q.shape[1] == 0:
+        raise ValueError(f"expected q [rows, a multiple of {h} heads, {d}], got {tuple(q.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"block attention expects bf16 or fp16 q, got {q.dtype}")
+    t, hq = q.shape[:2]
+    n = context_lens.numel()
+    _int32("context_lens", context_lens, (n,))
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.shape[0] != n or n == 0:
+        raise ValueError(f"block_tables must be int32 [{n}, blocks] for at least one sequence, got "
+                         f"{block_tables.dtype} {tuple(block_tables.shape)}")
+    width = block_tables.shape[1]
+    if width > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block_tables needs rows with contiguous entries")
+    if cu_seqlens is not None:
+        _int32("cu_seqlens", cu_seqlens, (n + 1,))
+    elif t != n or max_seqlen != 1:
+        raise ValueError(f"without cu_seqlens q has one row per sequence, got {t} rows for {n} sequences and "
+                         f"max_seqlen {max_seqlen}")
+    max_seqlen = int(max_seqlen)
+    if max_seqlen < 1:
+        raise ValueError(f"max_seqlen must be at least 1, got {max_seqlen}")
+    max_context = width * bs if max_context is None else int(max_context)
+    if max_context < 0:
+        raise ValueError(f"max_context must not be negative, got {max_context}")
+    if out is None:
+        out = torch.empty((t, hq, d), device=q.device, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
+            (out.stride(0) | out.stride(1)) % 4 or out.data_ptr() % 8:
+        raise ValueError("out must have q's shape and type, a contiguous head_dim and 8-byte aligned rows")
+    dev = _on_device("block_attention", q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out,
+                     *(() if cu_seqlens is None else (cu_seqlens,)))
+    if t == 0:
+        return out
+    q = _aligned_rows(q)
+    rows, tiles, splits = block_attention_plan(n * h, hq // h, max_seqlen, max_context)
+    # the splits' partials, the call's own: nothing is shared between streams or captured graphs
+    ws = (torch.empty(n * h * tiles * splits * rows * (d + 2), device=dev, dtype=torch.float32)
+          if splits > 1 else None)
+    _launch(dev, "fdms_block_attention", q.data_ptr(), nat.dtype_code(q.dtype), q.stride(0), q.stride(1), t,
+            k_cache.data_ptr(), v_cache.data_ptr(), int(k_cache.dtype != torch.int8), k_cache.stride(0),
+            k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(),
+            k_scale.stride(0), block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(),
+            nat.ptr(cu_seqlens), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), n, h, hq // h, d, nb, bs,
+            max_seqlen, rows, splits, d ** -0.5 if scale is None else float(scale))
+    return out

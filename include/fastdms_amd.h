@@ -609,6 +609,82 @@ int fdms_fused_decode_attention_planned(const void* q, int64_t qs_b, int64_t qs_
 int fdms_fp8_gemm(const void* x, int64_t x_s, const float* x_inv, const void* w, int64_t w_s, const float* w_inv,
                   const void* bias, void* y, int64_t y_s, int M, int N, int K, void* stream);
 
+/* Dense 8-bit block KV cache: the cache that keeps every token (the
+ * reference's dense paged path, fastdms/layers/attention.py:17-37, 94-100,
+ * keeps bf16 rows; 8 bits and block scales have no reference counterpart).
+ * Blocks of block_size tokens (16, 32, 64, 128 or 256) hold per kv head, in
+ * 8-bit codes (is_fp8 0: int8, -127 .. 127; 1: e4m3fn), K as rows
+ * [block_size][D] and V as tiles of 16 tokens, each transposed,
+ * [block_size / 16][D][16]; head_dim D is 64 or 128.  A head's part of a block
+ * is contiguous and 16-byte aligned; kc_b / kc_h / vc_b / vc_h are the strides
+ * of blocks and heads (multiples of 16).  k_scale / v_scale [blocks, heads]
+ * fp32 with block stride sc_b: a code stands for code * scale.  A slot is
+ * block * block_size + row, below 2^31.
+ *
+ * Block tables and slot map of a step from its lengths: sequence b (of at most
+ * 4096) holds cached_lens[b] tokens in the first ceil(cached / block_size)
+ * entries of its table row and gets new_lens[b]; the blocks it lacks are popped
+ * from free_blocks[0 .. *free_count), top first, in sequence order, and
+ * written to its row.  Token t < num_tokens gets slot_mapping[t] and
+ * positions[t] (-1 and 0 past the last token); cu_seqlens [num_seqs + 1],
+ * context_lens = cached + new, *free_count_out = what is left (not the same
+ * address as free_count).  *status is 0, or the sum of 1 (too few free
+ * blocks), 2 (a table row too narrow), 4 (num_tokens too small) and 8 (a
+ * negative length, a context from 2^31, or a count outside 0 ..
+ * num_free_blocks); then the tables are left alone, slots are -1, cu_seqlens
+ * 0, context_lens cached_lens and *free_count_out = *free_count. */
+int fdms_block_tables(const int32_t* cached_lens, const int32_t* new_lens, int num_seqs, int32_t* block_tables,
+                      int64_t bt_b, int width, const int32_t* free_blocks, int num_free_blocks,
+                      const int32_t* free_count, int block_size, int num_tokens, int32_t* slot_mapping,
+                      int64_t* positions, int32_t* cu_seqlens, int32_t* context_lens, int32_t* free_count_out,
+                      int32_t* status, void* stream);
+
+/* Store rows key / value [num_tokens, heads, D] (dtype fp32, fp16 or bf16,
+ * 16-byte aligned rows) at slot_mapping[t]; slots outside the cache are
+ * skipped.  Rows of one block must be neighbours with consecutive slots and
+ * follow the rows the block holds (several runs into one block in a call leave
+ * its contents undefined).  Scale of a (block, head): the least power of two s
+ * >= 2^-126 with max |x| <= 127 s or 448 s over the new rows, and no less than
+ * the block's scale if rows were there; codes x / s to nearest even; earlier
+ * rows' codes are rounded to a raised scale.  NaN is stored as 0, infinities
+ * saturate. */
+int fdms_store_block_kvcache(const void* key, const void* value, int dtype, int64_t ks_t, int64_t ks_h,
+                             int64_t vs_t, int64_t vs_h, void* k_cache, void* v_cache, int is_fp8, int64_t kc_b,
+                             int64_t kc_h, int64_t vc_b, int64_t vc_h, float* k_scale, float* v_scale, int64_t sc_b,
+                             const int32_t* slot_mapping, int num_tokens, int num_blocks, int block_size,
+                             int num_kv_heads, int head_dim, void* stream);
+
+/* Dense rows out_k / out_v [num_tokens, heads, D] (fp32, fp16 or bf16; even
+ * strides) = code * scale at slot_mapping[t], any order; a slot outside the
+ * cache gives zeros. */
+int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_fp8, int64_t kc_b, int64_t kc_h,
+                              int64_t vc_b, int64_t vc_h, const float* k_scale, const float* v_scale, int64_t sc_b,
+                              const int32_t* slot_mapping, int num_tokens, int num_blocks, int block_size,
+                              int num_kv_heads, int head_dim, void* out_k, void* out_v, int out_dtype, int64_t ok_t,
+                              int64_t ok_h, int64_t ov_t, int64_t ov_h, void* stream);
+
+/* Causal GQA attention over the cache (replaces flash_attn_with_kvcache and
+ * the paged flash_attn_varlen_func of attention.py:85-100): sequence b has
+ * query rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of q / out [total_rows, heads *
+ * group_size, D] (bf16 or fp16), the last of its context_lens[b] keys, which
+ * its table row (width entries, stride bt_b) leads to.  cu_seqlens NULL: one
+ * query row per sequence (total_rows = num_seqs, max_seqlen 1).  max_seqlen
+ * bounds the query rows of a sequence.  Contexts past what a table row can
+ * hold are cut; keys of a block outside the cache are left out; a query that
+ * sees no key gets zeros; rows outside cu_seqlens are not written.  q rows
+ * 16-byte, out rows 8-byte aligned.  tile_rows (16 or 32): query rows x heads
+ * per workgroup.  num_splits > 1 splits the keys; workspace then holds
+ * num_seqs * heads * ceil(max_seqlen * group_size / tile_rows) * num_splits *
+ * tile_rows * (D + 2) floats (16-byte aligned) that no other call may use
+ * meanwhile. */
+int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, int64_t qs_h, int total_rows,
+                         const void* k_cache, const void* v_cache, int is_fp8, int64_t kc_b, int64_t kc_h,
+                         int64_t vc_b, int64_t vc_h, const float* k_scale, const float* v_scale, int64_t sc_b,
+                         const int32_t* block_tables, int64_t bt_b, int width, const int32_t* context_lens,
+                         const int32_t* cu_seqlens, void* out, int64_t os_t, int64_t os_h, float* workspace,
+                         int num_seqs, int num_kv_heads, int group_size, int head_dim, int num_blocks,
+                         int block_size, int max_seqlen, int tile_rows, int num_splits, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
