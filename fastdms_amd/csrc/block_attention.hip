@@ -40,9 +40,11 @@ struct BlockAttnArgs {
   int64_t bt_b;
   const int32_t* context;
   const int32_t* cu;  // nullptr: one query row per sequence
-  float* part_o;      // [pair][tile][split][rows][D]
-  float* part_ml;     // [pair][tile][split][rows][2]
-  int width, num_blocks, shift, num_seqs, num_kv_heads, group, total_rows, splits, tiles;
+  float* part_o;    // [split][row of q][head][D], unnormalised
+  float* part_ml;   // [split][row of q][head][2]: maximum, sum
+  int* part_used;   // [row of q][head]: splits that hold a part of it
+  int width, num_blocks, shift, num_seqs, num_kv_heads, group, total_rows;
+  int few_rows;     // sequences of at most so many rows are block_attn_kernel's, longer ones the tile kernel's
   int q_f16;
   float scale;
 };
@@ -59,10 +61,15 @@ __device__ __forceinline__ SeqSpan seq_span(const BlockAttnArgs& a, int b) {
   return s;
 }
 
-// The splits a query tile uses of the launch's: at least four 64-key groups
-// each (one per wave), so a short context leaves the rest of its workgroups idle.
-__device__ __forceinline__ int splits_used(int groups, int splits) {
-  return min(splits, max(1, (groups + 3) >> 2));
+// The splits a query tile uses of the launch's: of at least `least` 64-key
+// groups each, so a short context leaves the rest of its workgroups idle.
+__device__ __forceinline__ int splits_used(int groups, int splits, int least) {
+  return min(splits, max(1, groups / least));
+}
+
+// Where a split's part of (row t of q, head) lies, in rows of D (part_o) or 2 (part_ml).
+__device__ __forceinline__ int64_t part_row(const BlockAttnArgs& a, int split, int t, int head) {
+  return ((int64_t)split * a.total_rows + t) * (a.num_kv_heads * a.group) + head;
 }
 
 __device__ __forceinline__ void store_out4(void* out, int64_t at, f32x4_t v, int f16) {
@@ -86,28 +93,26 @@ __device__ __forceinline__ float q_factor(float amax) {
   return __uint_as_float((uint32_t)(min(14 - e, 126) + 127) << 23);
 }
 
-// One workgroup: 16 * MT query rows (row r: token r / group, head r % group of
-// the kv head) of a sequence over one split of its keys; its four waves take
-// 64-key groups in turn and join at the end.
+// Sequences of few query rows (row r: token r / group, head r % group of the kv
+// head; at most 16 * MT).  One workgroup takes all of them over one split of
+// the keys; its four waves take 64-key groups in turn and join at the end.
 template <int D, bool FP8, int MT>
-__global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a) {
+__global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, int splits) {
   constexpr int KL = D / 64, DC = D / 16, KS = D / 32;  // K loads per row and lane, V row groups, K steps
   constexpr int ROWS = 16 * MT, PAD = D + 4;
   __shared__ float s_o[4][ROWS][PAD];
   __shared__ float s_ml[4][ROWS][2];
   const int pairs = a.num_seqs * a.num_kv_heads;
-  const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs, tile = blockIdx.y;
+  const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs;
   const int b = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
   const SeqSpan sp = seq_span(a, b);
-  const int rows = sp.n * a.group, row0 = tile * ROWS;
-  if (sp.n <= 0 || row0 >= rows) return;
+  if (sp.n <= 0 || sp.n > a.few_rows) return;
+  const int rows = sp.n * a.group;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int first_vis = sp.ctx - sp.n + 1;  // keys query 0 sees
-  const int last_row = min(row0 + ROWS, rows) - 1;
-  const int keys = min(sp.ctx, first_vis + last_row / a.group);  // keys the tile sees (may be <= 0)
-  const int full = first_vis + row0 / a.group;                   // keys that all of its rows see
-  const int groups = keys > 0 ? (keys + kGroupKeys - 1) / kGroupKeys : 0;
-  const int used = splits_used(groups, a.splits);
+  const int keys = sp.ctx, full = first_vis;  // keys that the last query sees, and that all of them see
+  const int groups = (keys + kGroupKeys - 1) / kGroupKeys;
+  const int used = splits_used(groups, splits, 4);
   if (split >= used) return;
   const int per = (groups + used - 1) / used;
   const int g_end = min(groups, (split + 1) * per);
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a) 
   int vis[MT];     // keys it sees
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int r = row0 + m * 16 + c;
+    const int r = m * 16 + c;
     const bool on = r < rows;
     const int i = on ? r / a.group : 0, hq = h * a.group + (on ? r % a.group : 0);
     vis[m] = on ? min(sp.ctx, first_vis + i) : 0;
@@ -220,7 +225,8 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a) 
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float x = st[m][t][r] * mul;
+#pragma clang fp contract(off)
+          float x = st[m][t][r] * mul;  // rounded, as the maximum taken of it is
           if (masked && !(okv && kv_v + 4 * t + r < vis[m])) x = kNegInf;
           st[m][t][r] = x;
           top = fmaxf(top, x);
@@ -271,8 +277,9 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a) 
   }
   __syncthreads();
   for (int e = tid; e < ROWS * (D / 4); e += 256) {
-    const int r = e / (D / 4), d = (e % (D / 4)) * 4, row = row0 + r;
-    if (row >= rows) break;
+    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+    if (r >= rows) break;
+    const int t = sp.q0 + r / a.group, head = h * a.group + r % a.group;
     float top = kNegInf;
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][r][0]);
@@ -287,61 +294,392 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a) 
     }
     if (used == 1) {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees no key: zeros
-      store_out4(a.out, (int64_t)(sp.q0 + row / a.group) * a.os_t + (int64_t)(h * a.group + row % a.group) * a.os_h + d,
-                 v * inv, a.q_f16);
+      store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
     } else {
-      const int64_t at = (((int64_t)pair * a.tiles + tile) * a.splits + split) * ROWS + r;
+      const int64_t at = part_row(a, split, t, head);
       *(f32x4_t*)(a.part_o + at * D + d) = v;
       if (d == 0) {
         a.part_ml[2 * at] = top;
         a.part_ml[2 * at + 1] = sum;
       }
     }
+    if (a.part_used && split == 0 && d == 0) a.part_used[part_row(a, 0, t, head)] = used;
+  }
+}
+
+// Sequences of many query rows: 128 rows of a kv head (128 / group tokens, all
+// of the group's heads) per workgroup, 32 per wave, over one split of the keys.
+//
+// 64 keys at a time go from the cache to LDS as halves, converted once by the
+// workgroup's four waves (wave w tile w) and read by each of them; two buffers,
+// one barrier per 64 keys, the codes of the next keys but one on their way in
+// registers meanwhile.  v_mfma_f32_32x32x16_f16 with S^T = K Q^T, O^T = V^T P^T:
+// a lane owns one query (column lane % 32).  V's 16 tokens are written in the
+// order in which a lane of a score tile holds them (0-3, 8-11, 4-7, 12-15), so
+// P goes from one product to the other in registers.
+//
+// The blocks' scales go into the halves: a block's codes times its scale over
+// the largest so far (a power of two no greater than 1 for the store's scales).
+// What falls below a half's range there is 2^-25 of that largest scale, far less than the fp32
+// sum it joins can hold next to it.  Then one factor holds for all keys of a
+// step, and exp(s - max) is one fma and one v_exp_f32 per score.
+//
+// A row's maximum is raised only when a score passes it by 2^8 (P stays below
+// 2^8, in a half's range): O is rescaled in the first steps and hardly again.
+constexpr int kTileRows = 128;
+constexpr float kLazyMax = 8.0f;
+
+__device__ __forceinline__ float half_max(float v) {  // over lanes l, l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Four codes as halves times a factor.
+template <bool FP8>
+__device__ __forceinline__ u32x2_t codes_scaled(uint32_t c, f16x2_t f) {
+  u32x2_t r;
+  uint32_t lo, hi;
+  codes_to_f16<FP8>(c, &lo, &hi);
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, lo) * f);
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, hi) * f);
+  return r;
+}
+
+// A 64-key step: the wave's tile (block id, -1: no such block or past the
+// keys, and scales), which of the four tiles are there and their largest scales.
+struct StepTiles {
+  int id;
+  float sk, sv, ktop, vtop;
+  unsigned there;
+};
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttnArgs a, int splits) {
+  constexpr int KSTEP = D / 16, DT = D / 32, KP = D / 64;
+  __shared__ u32x4_t s_k[2][64 * D / 8];  // 16-byte chunks, chunk c of row r at c ^ (r & 7)
+  __shared__ u32x4_t s_v[2][64 * D / 8];
+  const int pairs = a.num_seqs * a.num_kv_heads;
+  const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs;
+  const int b = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
+  const SeqSpan sp = seq_span(a, b);
+  if (sp.n <= a.few_rows) return;
+  const int rows = sp.n * a.group, tiles = (rows + kTileRows - 1) / kTileRows;
+  const int tile = tiles - 1 - (int)blockIdx.y;  // the tiles that see most keys first
+  if (tile < 0) return;
+  const int row0 = tile * kTileRows;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first_vis = sp.ctx - sp.n + 1;  // keys query 0 sees
+  const int keys = min(sp.ctx, first_vis + (min(row0 + kTileRows, rows) - 1) / a.group);  // that the tile sees
+  const int groups = keys > 0 ? (keys + kGroupKeys - 1) / kGroupKeys : 0;
+  const int used = splits_used(groups, splits, 8);
+  if (split >= used) return;
+  const int per = (groups + used - 1) / used;
+  const int g0 = split * per, g1 = min(groups, g0 + per);
+
+  // Q^T operand: channels 16 s + 8 half .. + 7 of row c
+  const int r = row0 + wave * 32 + c;
+  const bool on = r < rows;
+  const int t = sp.q0 + (on ? r / a.group : 0), head = h * a.group + (on ? r % a.group : 0);
+  const int vis = on ? min(sp.ctx, first_vis + r / a.group) : 0;
+  // keys that all / any of the wave's rows see
+  const int wfull = first_vis + (row0 + wave * 32) / a.group;
+  const int wrows = min(rows - (row0 + wave * 32), 32);
+  const int wkeys = wrows > 0 ? min(sp.ctx, first_vis + (row0 + wave * 32 + wrows - 1) / a.group) : 0;
+  f16x8_t qf[KSTEP];
+  float qmul;
+  {
+    const int64_t at = (int64_t)t * a.qs_t + (int64_t)head * a.qs_h;
+    u32x4_t raw[KSTEP];
+#pragma unroll
+    for (int s = 0; s < KSTEP; ++s) raw[s] = *(const u32x4_t*)((const uint16_t*)a.q + at + 16 * s + 8 * half);
+    float amax = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KSTEP; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t e = (raw[s][j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
+        amax = fmaxf(amax, fabsf(a.q_f16 ? (float)__builtin_bit_cast(f16_t, (uint16_t)e) : bf16_to_f32(e)));
+      }
+    const float f = q_factor(half_max(amax));
+    qmul = (fabsf(a.scale) * kLog2e) * (1.0f / f);
+    const float qf_mul = a.scale < 0.0f ? -f : f;  // the factor of the scores is positive: their maximum is the raw one's
+#pragma unroll
+    for (int s = 0; s < KSTEP; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t e = (raw[s][j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
+        qf[s][j] = (f16_t)((a.q_f16 ? (float)__builtin_bit_cast(f16_t, (uint16_t)e) : bf16_to_f32(e)) * qf_mul);
+      }
+  }
+
+  f32x16_t o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
+  float mx = kNegInf, l = 0.0f;
+
+  const int32_t* row_table = a.tables + (int64_t)b * a.bt_b;
+  const uint8_t* kbase = a.kc + (int64_t)h * a.kc_h;
+  const uint8_t* vbase = a.vc + (int64_t)h * a.vc_h;
+  const int bmask = (1 << a.shift) - 1;
+
+  auto tiles_of = [&](int gi) {
+    StepTiles s = {-1, 0.0f, 0.0f, 0.0f, 0.0f, 0u};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int key = gi * kGroupKeys + 16 * w;
+      const int id = (gi < g1 && key < keys) ? row_table[key >> a.shift] : -1;
+      if (id >= 0 && id < a.num_blocks) {
+        const int64_t at = (int64_t)id * a.sc_b + h;
+        const float sk = a.k_scale[at], sv = a.v_scale[at];
+        s.there |= 1u << w;
+        s.ktop = fmaxf(s.ktop, sk);
+        s.vtop = fmaxf(s.vtop, sv);
+        if (w == wave) {
+          s.id = id;
+          s.sk = sk;
+          s.sv = sv;
+        }
+      }
+    }
+    return s;
+  };
+  u32x4_t kr[KP], vr[KP];
+  auto load_codes = [&](int gi, const StepTiles& s) {
+    const int id = max(s.id, 0);
+    const int in_block = (gi * kGroupKeys + 16 * wave) & bmask;
+    const uint8_t* kp = kbase + (int64_t)id * a.kc_b + in_block * D + lane * 16;
+    const uint8_t* vp = vbase + (int64_t)id * a.vc_b + in_block * D + lane * 16;
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      kr[p] = *(const u32x4_t*)(kp + 1024 * p);
+      vr[p] = *(const u32x4_t*)(vp + 1024 * p);
+    }
+  };
+  // the wave's tile to LDS; ktop / vtop: the largest scales so far
+  auto write_codes = [&](int gi, int buf, const StepTiles& s, float ktop, float vtop) {
+    const f16_t fk = (f16_t)(s.sk / ktop), fv = (f16_t)(s.sv / vtop);
+    const f16x2_t fk2 = {fk, fk}, fv2 = {fv, fv};
+    const int live = s.id < 0 ? 0 : keys - (gi * kGroupKeys + 16 * wave);
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int at = lane + 64 * p, row = 16 * wave + at / (D / 16), chunk = 2 * (at % (D / 16));
+      u32x4_t w0, w1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x2_t x = codes_scaled<FP8>(kr[p][j], fk2), y = codes_scaled<FP8>(kr[p][2 + j], fk2);
+        w0[2 * j] = x[0], w0[2 * j + 1] = x[1], w1[2 * j] = y[0], w1[2 * j + 1] = y[1];
+      }
+      s_k[buf][row * (D / 8) + (chunk ^ (row & 7))] = w0;
+      s_k[buf][row * (D / 8) + ((chunk + 1) ^ (row & 7))] = w1;
+      // V: channel at of the tile; tokens past the keys may hold NaN codes, and 0 * NaN is no 0
+      if (live < kTile) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int nb = min(max(live - 4 * j, 0), 4);
+          vr[p][j] &= nb == 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x2_t x = codes_scaled<FP8>(vr[p][2 * j], fv2), y = codes_scaled<FP8>(vr[p][2 * j + 1], fv2);
+        w0[2 * j] = x[0], w0[2 * j + 1] = x[1], w1[2 * j] = y[0], w1[2 * j + 1] = y[1];
+      }
+      s_v[buf][at * 8 + ((2 * wave) ^ (at & 7))] = w0;
+      s_v[buf][at * 8 + ((2 * wave + 1) ^ (at & 7))] = w1;
+    }
+  };
+  float ktop = 1.17549435e-38f, vtop = 1.17549435e-38f;  // of the keys in the buffer being read
+  StepTiles cur = tiles_of(g0), nxt = tiles_of(g0 + 1);
+  if (g0 < g1) {
+    load_codes(g0, cur);
+    ktop = fmaxf(ktop, cur.ktop);
+    vtop = fmaxf(vtop, cur.vtop);
+    write_codes(g0, 0, cur, ktop, vtop);
+    load_codes(g0 + 1, nxt);
+  }
+  __syncthreads();
+  for (int gi = g0; gi < g1; ++gi) {
+    const int buf = (gi - g0) & 1, key0 = gi * kGroupKeys;
+    const bool busy = key0 < wkeys;
+    f32x16_t st[2];
+    if (busy) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) st[x][j] = 0.0f;
+        const int row = 32 * x + c;
+#pragma unroll
+        for (int s = 0; s < KSTEP; ++s) {
+          const f16x8_t kf = __builtin_bit_cast(f16x8_t, s_k[buf][row * (D / 8) + ((2 * s + half) ^ (row & 7))]);
+          st[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[x], 0, 0, 0);
+        }
+      }
+    }
+    // the next keys into the other buffer, those after them on their way
+    float ktop_n = ktop, vtop_n = vtop;
+    const unsigned there = cur.there;
+    if (gi + 1 < g1) {
+      ktop_n = fmaxf(ktop, nxt.ktop);
+      vtop_n = fmaxf(vtop, nxt.vtop);
+      write_codes(gi + 1, buf ^ 1, nxt, ktop_n, vtop_n);
+      cur = nxt;
+      nxt = tiles_of(gi + 2);
+      load_codes(gi + 2, nxt);
+    }
+    if (busy) {
+      if (there != 15u || key0 + kGroupKeys > wfull) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int key = 32 * x + 8 * (j >> 2) + 4 * half + (j & 3);
+            if (key0 + key >= vis || !((there >> (2 * x + (j >> 3))) & 1)) st[x][j] = kNegInf;
+          }
+      }
+      const float mul = fmaxf(qmul * ktop, 1e-37f);  // above 0: -inf stays -inf
+      float top = kNegInf;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, st[x][j]);
+      top = half_max(top) * mul;
+      if (__any(top > mx + kLazyMax)) {
+        const float mnew = fmaxf(mx, top);
+        const float alpha = __builtin_amdgcn_exp2f(mx - (mnew == kNegInf ? 0.0f : mnew));
+        mx = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= alpha;
+      }
+      const float base = mx == kNegInf ? 0.0f : mx;
+      // scores so large that the product's rounding, which base has and the fma has not, would show
+      if (__any(fabsf(base) > 65536.0f)) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float prod = st[x][j] * mul;
+            st[x][j] = prod - base;
+          }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) st[x][j] = __builtin_fmaf(st[x][j], mul, -base);
+      }
+      f16x8_t pf[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          f32x2_t p;
+          p[0] = __builtin_amdgcn_exp2f(st[x][j]);
+          p[1] = __builtin_amdgcn_exp2f(st[x][j + 1]);
+          const f16x2_t ph = __builtin_convertvector(p, f16x2_t);
+          const f16x2_t one = {(f16_t)1.0f, (f16_t)1.0f};
+          l = __builtin_amdgcn_fdot2(ph, one, l, false);
+          pf[2 * x + (j >> 3)][j & 7] = ph[0];
+          pf[2 * x + (j >> 3)][(j & 7) + 1] = ph[1];
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int row = 32 * d + c;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f16x8_t vf = __builtin_bit_cast(f16x8_t, s_v[buf][row * 8 + ((2 * u + half) ^ (row & 7))]);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[u], o[d], 0, 0, 0);
+        }
+      }
+    }
+    if (vtop_n > vtop) {
+      const float f = vtop / vtop_n;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    ktop = ktop_n;
+    vtop = vtop_n;
+    __syncthreads();
+  }
+
+  const float sum = half_sum(l);
+  if (!on) return;
+  const float inv = used > 1 ? vtop : (sum == 0.0f ? 0.0f : vtop / sum);  // a row that sees no key: zeros
+  const int64_t at = part_row(a, split, t, head);
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ch = 32 * d + 8 * j + 4 * half;
+      const f32x4_t v = f32x4_t{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]} * inv;
+      if (used > 1) *(f32x4_t*)(a.part_o + at * D + ch) = v;
+      else store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + ch, v, a.q_f16);
+    }
+  if (half == 0) {
+    if (used > 1) {
+      a.part_ml[2 * at] = mx;
+      a.part_ml[2 * at + 1] = sum;
+    }
+    if (a.part_used && split == 0) a.part_used[part_row(a, 0, t, head)] = used;
   }
 }
 
 // Joins the splits of the rows that used several: D / 4 lanes per row.
-template <int D, int ROWS>
-__global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArgs a) {
+template <int D>
+__global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArgs a, int splits) {
   constexpr int LPR = D / 4, RPG = 256 / LPR;
-  const int pair = blockIdx.x, b = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
-  const SeqSpan sp = seq_span(a, b);
-  const int rows = sp.n * a.group;
-  const int row = blockIdx.y * RPG + threadIdx.x / LPR, d = (threadIdx.x % LPR) * 4;
-  if (sp.n <= 0 || row >= rows) return;
-  const int tile = row / ROWS, last_row = min((tile + 1) * ROWS, rows) - 1;
-  const int keys = min(sp.ctx, sp.ctx - sp.n + 1 + last_row / a.group);
-  const int used = splits_used(keys > 0 ? (keys + kGroupKeys - 1) / kGroupKeys : 0, a.splits);
-  if (used == 1) return;
-  const int64_t at = ((int64_t)pair * a.tiles + tile) * a.splits * ROWS + row % ROWS;
+  const int heads = a.num_kv_heads * a.group;
+  const int64_t row = (int64_t)blockIdx.x * RPG + threadIdx.x / LPR;
+  const int d = (threadIdx.x % LPR) * 4;
+  const int t = (int)(row / heads), head = (int)(row % heads);
+  if (t >= a.total_rows) return;
+  if (a.cu && (t < a.cu[0] || t >= a.cu[a.num_seqs])) return;  // no sequence's row
+  const int used = min(a.part_used[row], splits);
+  if (used <= 1) return;
   float top = kNegInf;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * (at + (int64_t)s * ROWS)]);
+  for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * part_row(a, s, t, head)]);
   const float base = top == kNegInf ? 0.0f : top;
   float sum = 0.0f;
   f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s = 0; s < used; ++s) {
-    const int64_t p = at + (int64_t)s * ROWS;
+    const int64_t p = part_row(a, s, t, head);
     const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - base);
     sum += a.part_ml[2 * p + 1] * f;
     v += *(const f32x4_t*)(a.part_o + p * D + d) * f;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  store_out4(a.out, (int64_t)(sp.q0 + row / a.group) * a.os_t + (int64_t)(h * a.group + row % a.group) * a.os_h + d,
-             v * inv, a.q_f16);
+  store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
 }
 
 }  // namespace fdms
 
 using namespace fdms;
 
-template <int D, bool FP8, int MT>
-static int launch_block_attn(const BlockAttnArgs& a, int max_rows, hipStream_t st) {
-  const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads;
-  block_attn_kernel<D, FP8, MT><<<dim3((unsigned)(pairs * a.splits), a.tiles), 256, 0, st>>>(a);
-  FDMS_LAUNCH_CHECK();
-  if (a.splits > 1) {
-    constexpr int RPG = 256 / (D / 4);
-    block_attn_join_kernel<D, 16 * MT><<<dim3((unsigned)pairs, (max_rows - 1) / RPG + 1), 256, 0, st>>>(a);
+template <int D, bool FP8>
+static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, int tile_splits, hipStream_t st) {
+  const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads, max_rows = (int64_t)max_seqlen * a.group;
+  if (few_splits) {
+    const dim3 grid((unsigned)(pairs * few_splits));
+    if (a.few_rows * a.group <= 16) block_attn_kernel<D, FP8, 1><<<grid, 256, 0, st>>>(a, few_splits);
+    else block_attn_kernel<D, FP8, 2><<<grid, 256, 0, st>>>(a, few_splits);
+    FDMS_LAUNCH_CHECK();
+  }
+  if (tile_splits) {
+    const dim3 grid((unsigned)(pairs * tile_splits), (unsigned)((max_rows - 1) / kTileRows + 1));
+    block_attn_tile_kernel<D, FP8><<<grid, 256, 0, st>>>(a, tile_splits);
+    FDMS_LAUNCH_CHECK();
+  }
+  const int splits = few_splits > tile_splits ? few_splits : tile_splits;
+  if (splits > 1) {
+    const int64_t rows = (int64_t)a.total_rows * a.num_kv_heads * a.group, per = 256 / (D / 4);
+    block_attn_join_kernel<D><<<dim3((unsigned)((rows - 1) / per + 1)), 256, 0, st>>>(a, splits);
     FDMS_LAUNCH_CHECK();
   }
   return 0;
@@ -353,20 +691,26 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
                                      int64_t sc_b, const int32_t* block_tables, int64_t bt_b, int width,
                                      const int32_t* context_lens, const int32_t* cu_seqlens, void* out, int64_t os_t,
                                      int64_t os_h, float* workspace, int num_seqs, int num_kv_heads, int group_size,
-                                     int head_dim, int num_blocks, int block_size, int max_seqlen, int tile_rows,
-                                     int num_splits, float scale, void* stream) {
+                                     int head_dim, int num_blocks, int block_size, int max_seqlen, int few_rows,
+                                     int few_splits, int tile_splits, float scale, void* stream) {
   if ((q_dtype != kF16 && q_dtype != kBF16) || total_rows < 0 || num_seqs < 1 || num_kv_heads < 1 || group_size < 1 ||
       (head_dim != 64 && head_dim != 128) || max_seqlen < 1 || width < 0 || num_blocks < 1 || block_size < 16 ||
-      block_size > 256 || (block_size & (block_size - 1)) || num_splits < 1 || num_splits > 1024 ||
-      (tile_rows != 16 && tile_rows != 32) || (num_splits > 1 && workspace == nullptr) ||
+      block_size > 256 || (block_size & (block_size - 1)) ||
       (cu_seqlens == nullptr && (max_seqlen != 1 || total_rows != num_seqs)))
+    return (int)hipErrorInvalidValue;
+  // every sequence length has its kernel: up to few_rows query rows the one, past them the other
+  const int splits = few_splits > tile_splits ? few_splits : tile_splits;
+  if (few_rows < 0 || (int64_t)few_rows * group_size > 32 || few_splits < 0 || tile_splits < 0 || splits < 1 ||
+      splits > 1024 || (few_rows > 0 && few_splits == 0) || (few_rows < max_seqlen && tile_splits == 0) ||
+      (splits > 1 && workspace == nullptr))
     return (int)hipErrorInvalidValue;
   if (!fdms_aligned16(q, k_cache, v_cache, workspace) || (uintptr_t)out % 8 || qs_t % 8 || qs_h % 8 || os_t % 4 ||
       os_h % 4 || kc_b % 16 || kc_h % 16 || vc_b % 16 || vc_h % 16)
     return (int)hipErrorInvalidValue;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads, max_rows = (int64_t)max_seqlen * group_size;
-  const int64_t tiles = (max_rows - 1) / tile_rows + 1;
-  if (pairs * num_splits > 0x7FFFFFFF || tiles > 65535 || (int64_t)total_rows * group_size > 0x7FFFFFFF)
+  const int64_t rows = (int64_t)total_rows * num_kv_heads * group_size;
+  if (pairs * splits > 0x7FFFFFFF || (max_rows - 1) / kTileRows + 1 > 65535 || max_rows > 0x7FFFFFFF ||
+      (int64_t)total_rows * group_size > 0x7FFFFFFF || rows > 0x7FFFFFFFll * 4)
     return (int)hipErrorInvalidValue;
   if (total_rows == 0) return 0;
   BlockAttnArgs a;
@@ -377,14 +721,14 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   a.k_scale = k_scale, a.v_scale = v_scale, a.sc_b = sc_b;
   a.tables = block_tables, a.bt_b = bt_b, a.width = width;
   a.context = context_lens, a.cu = cu_seqlens;
-  a.part_o = workspace, a.part_ml = workspace + pairs * tiles * num_splits * tile_rows * head_dim;
+  a.part_o = workspace;
+  a.part_ml = workspace + splits * rows * head_dim;
+  a.part_used = splits > 1 ? (int*)(a.part_ml + splits * rows * 2) : nullptr;
   a.num_blocks = num_blocks, a.shift = __builtin_ctz(block_size), a.num_seqs = num_seqs;
   a.num_kv_heads = num_kv_heads, a.group = group_size, a.total_rows = total_rows;
-  a.splits = num_splits, a.tiles = (int)tiles, a.q_f16 = q_dtype == kF16, a.scale = scale;
+  a.few_rows = few_rows, a.q_f16 = q_dtype == kF16, a.scale = scale;
   hipStream_t st = (hipStream_t)stream;
-  const int rows = (int)max_rows;
-#define FDMS_ATTN(D, F) \
-  return tile_rows == 16 ? launch_block_attn<D, F, 1>(a, rows, st) : launch_block_attn<D, F, 2>(a, rows, st)
+#define FDMS_ATTN(D, F) return launch_block_attn<D, F>(a, max_seqlen, few_splits, tile_splits, st)
   if (head_dim == 64) {
     if (is_fp8) FDMS_ATTN(64, true);
     FDMS_ATTN(64, false);

@@ -236,16 +236,28 @@ def gather_block_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: 
     return k, v
 
 
-def block_attention_plan(pairs: int, group: int, max_seqlen: int, max_context: int) -> tuple[int, int, int]:
-    """(query rows per tile, tiles, splits of the keys) of a block_attention
-    launch over ``pairs`` (sequence, kv head) pairs: tiles of 16 rows, or 32
-    when a sequence has more; splits to reach about four workgroups per CU,
-    each of at least 256 keys of the longest context."""
-    max_rows = max_seqlen * group
-    rows = 16 if max_rows <= 16 else 32
-    tiles = -(-max_rows // rows)
-    splits = min(-(-1024 // (pairs * tiles)), -(-max_context // 256), 256)
-    return rows, tiles, max(1, splits)
+def block_attention_plan(seqs: int, heads: int, group: int, rows: int, max_seqlen: int,
+                         max_context: int) -> tuple[int, int, int]:
+    """(few_rows, few_splits, tile_splits) of a block_attention launch over
+    ``rows`` query rows: sequences of up to few_rows rows go to the kernel for
+    few rows, longer ones to the one for many; 0 splits leave a launch out.
+
+    A batch whose longest run has at most 32 rows x heads takes the first
+    kernel alone, one sequence of more the second alone; several sequences may
+    be of both kinds, and the first then takes those of at most 16.  Splits:
+    the first kernel to four workgroups per CU, each of at least 256 keys of
+    the longest context; the second to two per CU over the tiles that ``rows``
+    can make, each of at least 512 keys."""
+    pairs = seqs * heads
+    if max_seqlen * group <= 32:
+        few_rows = max_seqlen
+    else:
+        few_rows = 16 // group if seqs > 1 else 0
+    few = max(1, min(-(-1024 // pairs), -(-max_context // 256), 256)) if few_rows else 0
+    if few_rows >= max_seqlen:
+        return few_rows, few, 0
+    tiles = heads * (rows * group // 128 + seqs)
+    return few_rows, few, max(1, min(-(-512 // tiles), -(-max_context // 512), 32))
 
 
 def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -299,14 +311,14 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if t == 0:
         return out
     q = _aligned_rows(q)
-    rows, tiles, splits = block_attention_plan(n * h, hq // h, max_seqlen, max_context)
+    few_rows, few_splits, tile_splits = block_attention_plan(n, h, hq // h, t, max_seqlen, max_context)
+    splits = max(few_splits, tile_splits)
     # the splits' partials, the call's own: nothing is shared between streams or captured graphs
-    ws = (torch.empty(n * h * tiles * splits * rows * (d + 2), device=dev, dtype=torch.float32)
-          if splits > 1 else None)
+    ws = torch.empty(t * hq * (splits * (d + 2) + 1), device=dev, dtype=torch.float32) if splits > 1 else None
     _launch(dev, "fdms_block_attention", q.data_ptr(), nat.dtype_code(q.dtype), q.stride(0), q.stride(1), t,
             k_cache.data_ptr(), v_cache.data_ptr(), int(k_cache.dtype != torch.int8), k_cache.stride(0),
             k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(),
             k_scale.stride(0), block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(),
             nat.ptr(cu_seqlens), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), n, h, hq // h, d, nb, bs,
-            max_seqlen, rows, splits, d ** -0.5 if scale is None else float(scale))
+            max_seqlen, few_rows, few_splits, tile_splits, d ** -0.5 if scale is None else float(scale))
     return out

@@ -672,18 +672,21 @@ int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_f
  * bounds the query rows of a sequence.  Contexts past what a table row can
  * hold are cut; keys of a block outside the cache are left out; a query that
  * sees no key gets zeros; rows outside cu_seqlens are not written.  q rows
- * 16-byte, out rows 8-byte aligned.  tile_rows (16 or 32): query rows x heads
- * per workgroup.  num_splits > 1 splits the keys; workspace then holds
- * num_seqs * heads * ceil(max_seqlen * group_size / tile_rows) * num_splits *
- * tile_rows * (D + 2) floats (16-byte aligned) that no other call may use
- * meanwhile. */
+ * 16-byte, out rows 8-byte aligned.  Sequences of up to few_rows
+ * query rows (few_rows * group_size <= 32) run on the kernel for few rows with
+ * their keys in up to few_splits parts, longer ones on the one for many with
+ * up to tile_splits; a count of 0 leaves a launch out and is refused where a
+ * sequence may need it.  With S the larger count above 1 the workspace holds
+ * S * total_rows * heads * group_size * (D + 2) + total_rows * heads *
+ * group_size floats (16-byte aligned) that no other call may use meanwhile. */
 int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, int64_t qs_h, int total_rows,
                          const void* k_cache, const void* v_cache, int is_fp8, int64_t kc_b, int64_t kc_h,
                          int64_t vc_b, int64_t vc_h, const float* k_scale, const float* v_scale, int64_t sc_b,
                          const int32_t* block_tables, int64_t bt_b, int width, const int32_t* context_lens,
                          const int32_t* cu_seqlens, void* out, int64_t os_t, int64_t os_h, float* workspace,
                          int num_seqs, int num_kv_heads, int group_size, int head_dim, int num_blocks,
-                         int block_size, int max_seqlen, int tile_rows, int num_splits, float scale, void* stream);
+                         int block_size, int max_seqlen, int few_rows, int few_splits, int tile_splits,
+                         float scale, void* stream);
 
 #ifdef __cplusplus
 }

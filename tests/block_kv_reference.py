@@ -102,6 +102,9 @@ def attention(q, cache: Cache, table, context, cu, scale=None):
       range; sums and products of fp32 add a few 2^-24 per term and the scores'
       own error e_s = |s| * (D + 8) * 2^-24 shifts exp(s) by e_s of itself:
       sum_j p_j |v_j| * (2^-11 + 2 e_s + n 2^-24) + n 2^-25 max |v|, over sum p;
+    * codes may be held as halves relative to the largest scale of the
+      sequence, and then are off by at most 2^-25 of it: e_s grows by scale *
+      2^-25 max sK * sum |q|, the result by 2^-25 max sV;
     * the result is rounded once to its type: eps / 2 of itself."""
     t, hq, d = q.shape
     nb, h = cache.scale["k"].shape
@@ -120,6 +123,8 @@ def attention(q, cache: Cache, table, context, cu, scale=None):
                  for p in range(ctx)]
         here = torch.tensor([s >= 0 for s in slots], dtype=torch.bool)
         k, v = cache.rows("k", slots), cache.rows("v", slots)
+        blocks = [x for x in table[b][:math.ceil(ctx / cache.bs)] if 0 <= x < nb]
+        tops = [[float(cache.scale[x][blocks, j].max()) if blocks else 0.0 for j in range(h)] for x in ("k", "v")]
         for i in range(q1 - q0):
             last = ctx - (q1 - q0) + i
             seen = here & (torch.arange(ctx) <= last)
@@ -133,9 +138,11 @@ def attention(q, cache: Cache, table, context, cu, scale=None):
                 o = p @ vv[:, j // g]
                 a = p @ vv[:, j // g].abs()
                 es = float(s.abs().max()) * (d + 8) * 2.0 ** -24
+                es += abs(scale) * 2.0 ** -25 * tops[0][j // g] * float(q[q0 + i, j].abs().sum())
                 top = float(p.max())
                 out[q0 + i, j] = o
                 err = a * (2.0 ** -11 + 2 * es + n * 2.0 ** -24) + top * n * 2.0 ** -25 * float(vv.abs().max())
+                err = err + 2.0 ** -25 * tops[1][j // g]
                 bound[q0 + i, j] = err + half * (o.abs() + err)
     return out, bound
 

@@ -334,62 +334,71 @@ def test_attention_query_runs(dtype, d, context, lens):
 def test_attention_queries_that_see_no_key():
     """More queries than keys: the first ones see nothing and get zeros; a context of none gives zeros."""
     cache, table = _attend_case(16, 1, 64, FP8, [3, 0])
-    got = _check_attention(cache, table, [3, 0], [10, 4], 2)
-    assert (got[:7] == 0).all() and (got[10:] == 0).all() and (got[7:10] != 0).any()
+    for n in (10, 200):
+        got = _check_attention(cache, table, [3, 0], [n, n // 2], 2)
+        assert (got[:n - 3] == 0).all() and (got[n:] == 0).all() and (got[n - 3:n] != 0).any()
 
 
 @pytest.mark.parametrize("dtype", [torch.int8, FP8])
-def test_attention_blocks_that_are_not_there(dtype):
+@pytest.mark.parametrize("lens", [[2, 3, 1], [50, 45, 20]])
+def test_attention_blocks_that_are_not_there(dtype, lens):
     """Entries of -1 or past the cache leave their keys out; contexts past the table's row are cut."""
     cache, table = _attend_case(16, 2, 64, dtype, [100, 90, 64])
     nb = cache[0].shape[0]
     table[0][2], table[1][0], table[1][1] = -1, nb, 2 ** 31 - 1
     table[2] = [-5] * len(table[2])
-    got = _check_attention(cache, table, [100, 90, 64], [2, 3, 1], 4)
-    assert (got[5] == 0).all()
+    got = _check_attention(cache, table, [100, 90, 64], lens, 4)
+    assert (got[lens[0] + lens[1]:] == 0).all()
     cut = [r[:4] for r in table]
-    _check_attention(cache, cut, [100, 90, 64], [2, 3, 1], 4)
+    _check_attention(cache, cut, [100, 90, 64], lens, 4)
 
 
 @pytest.mark.parametrize("q_dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("scale", [None, 0.3, -0.2, 0.0])
-def test_attention_types_and_scales(q_dtype, scale):
+@pytest.mark.parametrize("lens", [[1, 4], [3, 50]])
+def test_attention_types_and_scales(q_dtype, scale, lens):
     cache, table = _attend_case(32, 2, 128, torch.int8, [77, 200])
-    _check_attention(cache, table, [77, 200], [1, 4], 4, dtype=q_dtype, scale=scale)
+    _check_attention(cache, table, [77, 200], lens, 4, dtype=q_dtype, scale=scale)
 
 
-def test_attention_large_and_tiny_queries():
+@pytest.mark.parametrize("n", [6, 42])
+def test_attention_large_and_tiny_queries(n):
     """Query magnitudes that a half could not hold, row by row."""
     cache, table = _attend_case(16, 2, 64, FP8, [130])
-    q = torch.randn((6, 4, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
-    q *= torch.tensor([1e30, 1e-30, 1e5, 1e-8, 0.0, 1.0], device=DEV)[:, None, None]
+    q = torch.randn((n, 4, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    q *= torch.tensor([1e30, 1e-30, 1e5, 1e-8, 0.0, 1.0] * (n // 6), device=DEV)[:, None, None]
     q[0] *= 1e-30 / 3e-1
     k = cache[2]
     k *= torch.tensor(2.0 ** -6, device=DEV)  # keep the scores of the large rows moderate
-    _check_attention(cache, table, [130], [6], 2, q=q.bfloat16())
+    _check_attention(cache, table, [130], [n], 2, q=q.bfloat16())
 
 
-def test_attention_scales_that_differ_widely():
+@pytest.mark.parametrize("n", [1, 100])
+def test_attention_scales_that_differ_widely(n):
     """V scales from 2^-40 to 2^40 in one context: the small blocks' part is lost only below the bound."""
     cache, table = _attend_case(16, 1, 64, torch.int8, [16 * 9])
     cache[3].copy_(torch.exp2(torch.linspace(-40, 40, cache[3].numel(), device=DEV).round()).view_as(cache[3]))
-    _check_attention(cache, table, [16 * 9], [1], 4)
+    _check_attention(cache, table, [16 * 9], [n], 4)
+    cache[2].copy_(torch.exp2(torch.linspace(-30, -3, cache[2].numel(), device=DEV).round()).view_as(cache[2]))
+    _check_attention(cache, table, [16 * 9], [n], 4)
 
 
-def test_attention_row_of_nan_or_infinite_query_leaves_the_others():
+@pytest.mark.parametrize("n", [4, 36])
+def test_attention_row_of_nan_or_infinite_query_leaves_the_others(n):
     cache, table = _attend_case(16, 1, 64, torch.int8, [50])
-    q = torch.randn((4, 2, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
-    clean = _check_attention(cache, table, [50], [4], 2, q=q)
+    q = torch.randn((n, 2, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
+    clean = _check_attention(cache, table, [50], [n], 2, q=q)
     bad = q.clone()
-    bad[1, 0, 5] = float("nan")
-    bad[2, 1, 7] = float("inf")
-    got = _kv().block_attention(bad, *cache, _ints(table), _ints([50]), cu_seqlens=_ints([0, 4]), max_seqlen=4)
-    assert got[1, 0].isnan().all() and not got[2, 1].isfinite().all()
-    for i, j in ((0, 0), (0, 1), (1, 1), (2, 0), (3, 0), (3, 1)):
-        assert torch.equal(got[i, j], clean[i, j])
+    bad[n - 3, 0, 5] = float("nan")
+    bad[n - 2, 1, 7] = float("inf")
+    got = _kv().block_attention(bad, *cache, _ints(table), _ints([50]), cu_seqlens=_ints([0, n]), max_seqlen=n)
+    assert got[n - 3, 0].isnan().all() and not got[n - 2, 1].isfinite().all()
+    same = torch.ones((n, 2), dtype=torch.bool)
+    same[n - 3, 0] = same[n - 2, 1] = False
+    assert torch.equal(got.cpu()[same], clean.cpu()[same])
 
 
-@pytest.mark.parametrize("lens", [[1, 1], [6, 3]])
+@pytest.mark.parametrize("lens", [[1, 1], [6, 3], [2, 40], [70, 3]])
 def test_attention_long_context_splits(lens):
     """Contexts that many workgroups share, one far shorter than the other."""
     context = [9001, 40]
