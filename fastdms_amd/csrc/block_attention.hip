@@ -73,15 +73,21 @@ __device__ __forceinline__ int64_t part_row(const BlockAttnArgs& a, int split, i
 }
 
 __device__ __forceinline__ void store_out4(void* out, int64_t at, f32x4_t v, int f16) {
-  u32x2_t r;
-  if (f16) {
-    const f16x4_t h = __builtin_convertvector(v, f16x4_t);
-    r = __builtin_bit_cast(u32x2_t, h);
-  } else {
-    r[0] = f32_to_bf16(v[0]) | (f32_to_bf16(v[1]) << 16);
-    r[1] = f32_to_bf16(v[2]) | (f32_to_bf16(v[3]) << 16);
-  }
+  typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+  const u32x2_t h = __builtin_bit_cast(u32x2_t, __builtin_convertvector(v, f16x4_t));
+  const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_convertvector(v, bf16x4_t));  // v_cvt_pk_bf16_f32
+  const u32x2_t r = f16 ? h : b;
   *(u32x2_t*)((uint16_t*)out + at) = r;
+}
+
+// Eight fp16 or bf16 values; both read without a branch.
+__device__ __forceinline__ void halves_to_f32(u32x4_t raw, int f16, float* x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t e = raw[j >> 1] >> (16 * (j & 1));
+    const float as_half = (float)__builtin_bit_cast(f16_t, (uint16_t)e), as_bf16 = bf16_to_f32(e & 0xFFFFu);
+    x[j] = __uint_as_float(f16 ? __float_as_uint(as_half) : __float_as_uint(as_bf16));
+  }
 }
 
 // Power of two that brings a row of largest magnitude amax near 2^14, so the
@@ -132,12 +138,9 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const u32x4_t raw = *(const u32x4_t*)((const uint16_t*)a.q + at + (s >> 1) * 64 + g * 16 + (s & 1) * 8);
+      halves_to_f32(raw, a.q_f16, x[s]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t e = (raw[j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-        x[s][j] = a.q_f16 ? (float)__builtin_bit_cast(f16_t, (uint16_t)e) : bf16_to_f32(e);
-        amax = fmaxf(amax, fabsf(x[s][j]));
-      }
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
     }
     const float f = q_factor(rows_max(amax));
     qmul[m] = (a.scale * kLog2e) * (1.0f / f);
@@ -349,13 +352,15 @@ __device__ __forceinline__ u32x2_t codes_scaled(uint32_t c, f16x2_t f) {
   return r;
 }
 
-// A 64-key step: the wave's tile (block id, -1: no such block or past the
-// keys, and scales), which of the four tiles are there and their largest scales.
+// A 64-key step's four tiles, in lanes: lane i holds tile i % 4.
 struct StepTiles {
-  int id;
-  float sk, sv, ktop, vtop;
-  unsigned there;
+  int id;        // block, -1: no such block or past the keys
+  float sk, sv;  // its scales
 };
+__device__ __forceinline__ float quad_max(float v) {  // over the four tiles
+  v = fmaxf(v, dpp_mov_f<0xB1>(v));
+  return fmaxf(v, dpp_mov_f<0x4E>(v));
+}
 
 template <int D, bool FP8>
 __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttnArgs a, int splits) {
@@ -397,24 +402,20 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
     u32x4_t raw[KSTEP];
 #pragma unroll
     for (int s = 0; s < KSTEP; ++s) raw[s] = *(const u32x4_t*)((const uint16_t*)a.q + at + 16 * s + 8 * half);
-    float amax = 0.0f;
+    float x[KSTEP][8], amax = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KSTEP; ++s)
+    for (int s = 0; s < KSTEP; ++s) {
+      halves_to_f32(raw[s], a.q_f16, x[s]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t e = (raw[s][j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-        amax = fmaxf(amax, fabsf(a.q_f16 ? (float)__builtin_bit_cast(f16_t, (uint16_t)e) : bf16_to_f32(e)));
-      }
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
+    }
     const float f = q_factor(half_max(amax));
     qmul = (fabsf(a.scale) * kLog2e) * (1.0f / f);
     const float qf_mul = a.scale < 0.0f ? -f : f;  // the factor of the scores is positive: their maximum is the raw one's
 #pragma unroll
     for (int s = 0; s < KSTEP; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t e = (raw[s][j >> 1] >> (16 * (j & 1))) & 0xFFFFu;
-        qf[s][j] = (f16_t)((a.q_f16 ? (float)__builtin_bit_cast(f16_t, (uint16_t)e) : bf16_to_f32(e)) * qf_mul);
-      }
+      for (int j = 0; j < 8; ++j) qf[s][j] = (f16_t)(x[s][j] * qf_mul);
   }
 
   f32x16_t o[DT];
@@ -429,30 +430,20 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
   const uint8_t* vbase = a.vc + (int64_t)h * a.vc_h;
   const int bmask = (1 << a.shift) - 1;
 
-  auto tiles_of = [&](int gi) {
-    StepTiles s = {-1, 0.0f, 0.0f, 0.0f, 0.0f, 0u};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int key = gi * kGroupKeys + 16 * w;
-      const int id = (gi < g1 && key < keys) ? row_table[key >> a.shift] : -1;
-      if (id >= 0 && id < a.num_blocks) {
-        const int64_t at = (int64_t)id * a.sc_b + h;
-        const float sk = a.k_scale[at], sv = a.v_scale[at];
-        s.there |= 1u << w;
-        s.ktop = fmaxf(s.ktop, sk);
-        s.vtop = fmaxf(s.vtop, sv);
-        if (w == wave) {
-          s.id = id;
-          s.sk = sk;
-          s.sv = sv;
-        }
-      }
-    }
-    return s;
+  const int quad16 = 16 * (lane & 3);
+  auto ids_of = [&](int gi) {
+    const int key = gi * kGroupKeys + quad16;
+    const int id = row_table[min(key, keys - 1) >> a.shift];
+    return gi < g1 && key < keys && id < a.num_blocks ? id : -1;
+  };
+  auto scales_of = [&](int id) {
+    const int64_t at = (int64_t)max(id, 0) * a.sc_b + h;
+    const float sk = a.k_scale[at], sv = a.v_scale[at];
+    return StepTiles{id, id < 0 ? 0.0f : sk, id < 0 ? 0.0f : sv};
   };
   u32x4_t kr[KP], vr[KP];
-  auto load_codes = [&](int gi, const StepTiles& s) {
-    const int id = max(s.id, 0);
+  auto load_codes = [&](int gi, int ids) {
+    const int id = max(__builtin_amdgcn_readlane(ids, wave), 0);
     const int in_block = (gi * kGroupKeys + 16 * wave) & bmask;
     const uint8_t* kp = kbase + (int64_t)id * a.kc_b + in_block * D + lane * 16;
     const uint8_t* vp = vbase + (int64_t)id * a.vc_b + in_block * D + lane * 16;
@@ -464,9 +455,12 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
   };
   // the wave's tile to LDS; ktop / vtop: the largest scales so far
   auto write_codes = [&](int gi, int buf, const StepTiles& s, float ktop, float vtop) {
-    const f16_t fk = (f16_t)(s.sk / ktop), fv = (f16_t)(s.sv / vtop);
+    const float sk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s.sk), wave));
+    const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s.sv), wave));
+    const int id = __builtin_amdgcn_readlane(s.id, wave);
+    const f16_t fk = (f16_t)(sk * __builtin_amdgcn_rcpf(ktop)), fv = (f16_t)(sv * __builtin_amdgcn_rcpf(vtop));
     const f16x2_t fk2 = {fk, fk}, fv2 = {fv, fv};
-    const int live = s.id < 0 ? 0 : keys - (gi * kGroupKeys + 16 * wave);
+    const int live = id < 0 ? 0 : keys - (gi * kGroupKeys + 16 * wave);
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int at = lane + 64 * p, row = 16 * wave + at / (D / 16), chunk = 2 * (at % (D / 16));
@@ -496,13 +490,18 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
     }
   };
   float ktop = 1.17549435e-38f, vtop = 1.17549435e-38f;  // of the keys in the buffer being read
-  StepTiles cur = tiles_of(g0), nxt = tiles_of(g0 + 1);
+  StepTiles cur = {-1, 0.0f, 0.0f}, nxt = cur;
+  int ids2 = -1;  // of the step after next
   if (g0 < g1) {
-    load_codes(g0, cur);
-    ktop = fmaxf(ktop, cur.ktop);
-    vtop = fmaxf(vtop, cur.vtop);
+    const int ids0 = ids_of(g0), ids1 = ids_of(g0 + 1);
+    ids2 = ids_of(g0 + 2);
+    cur = scales_of(ids0);
+    nxt = scales_of(ids1);
+    load_codes(g0, ids0);
+    ktop = fmaxf(ktop, quad_max(cur.sk));
+    vtop = fmaxf(vtop, quad_max(cur.sv));
     write_codes(g0, 0, cur, ktop, vtop);
-    load_codes(g0 + 1, nxt);
+    load_codes(g0 + 1, ids1);
   }
   __syncthreads();
   for (int gi = g0; gi < g1; ++gi) {
@@ -510,28 +509,37 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
     const bool busy = key0 < wkeys;
     f32x16_t st[2];
     if (busy) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int j = 0; j < 16; ++j) st[x][j] = 0.0f;
-        const int row = 32 * x + c;
 #pragma unroll
-        for (int s = 0; s < KSTEP; ++s) {
-          const f16x8_t kf = __builtin_bit_cast(f16x8_t, s_k[buf][row * (D / 8) + ((2 * s + half) ^ (row & 7))]);
-          st[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], st[x], 0, 0, 0);
-        }
+      for (int s0 = 0; s0 < KSTEP; s0 += 4) {  // eight operands on their way at once
+        f16x8_t kf[4][2];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            kf[s][x] = __builtin_bit_cast(
+                f16x8_t, s_k[buf][(32 * x + c) * (D / 8) + ((2 * (s0 + s) + half) ^ (c & 7))]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            st[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s][x], qf[s0 + s], st[x], 0, 0, 0);
       }
     }
     // the next keys into the other buffer, those after them on their way
     float ktop_n = ktop, vtop_n = vtop;
-    const unsigned there = cur.there;
+    const unsigned there = (unsigned)__ballot(cur.id >= 0) & 15u;
     if (gi + 1 < g1) {
-      ktop_n = fmaxf(ktop, nxt.ktop);
-      vtop_n = fmaxf(vtop, nxt.vtop);
+      ktop_n = fmaxf(ktop, quad_max(nxt.sk));
+      vtop_n = fmaxf(vtop, quad_max(nxt.sv));
       write_codes(gi + 1, buf ^ 1, nxt, ktop_n, vtop_n);
       cur = nxt;
-      nxt = tiles_of(gi + 2);
-      load_codes(gi + 2, nxt);
+      nxt = scales_of(ids2);
+      load_codes(gi + 2, ids2);
+      ids2 = ids_of(gi + 3);
     }
     if (busy) {
       if (there != 15u || key0 + kGroupKeys > wfull) {
@@ -575,7 +583,14 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
 #pragma unroll
           for (int j = 0; j < 16; ++j) st[x][j] = __builtin_fmaf(st[x][j], mul, -base);
       }
-      f16x8_t pf[4];
+      f16x8_t pf[4], vf[2][4];
+      auto load_v = [&](int d) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          vf[d & 1][u] = __builtin_bit_cast(f16x8_t, s_v[buf][(32 * d + c) * 8 + ((2 * u + half) ^ (c & 7))]);
+      };
+      load_v(0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -591,16 +606,14 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
         }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const int row = 32 * d + c;
+        if (d + 1 < DT) load_v(d + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const f16x8_t vf = __builtin_bit_cast(f16x8_t, s_v[buf][row * 8 + ((2 * u + half) ^ (row & 7))]);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[u], o[d], 0, 0, 0);
-        }
+        for (int u = 0; u < 4; ++u) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d & 1][u], pf[u], o[d], 0, 0, 0);
       }
     }
     if (vtop_n > vtop) {
-      const float f = vtop / vtop_n;
+      const float f = vtop * __builtin_amdgcn_rcpf(vtop_n);
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
     }

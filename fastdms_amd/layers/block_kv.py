@@ -246,8 +246,9 @@ def block_attention_plan(seqs: int, heads: int, group: int, rows: int, max_seqle
     kernel alone, one sequence of more the second alone; several sequences may
     be of both kinds, and the first then takes those of at most 16.  Splits:
     the first kernel to four workgroups per CU, each of at least 256 keys of
-    the longest context; the second to two per CU over the tiles that ``rows``
-    can make, each of at least 512 keys."""
+    the longest context; the second those, each of at least 512 keys, that take
+    the least rounds x keys of the 512 workgroups (two per CU) the chip holds,
+    over the tiles that ``rows`` can make."""
     pairs = seqs * heads
     if max_seqlen * group <= 32:
         few_rows = max_seqlen
@@ -257,7 +258,8 @@ def block_attention_plan(seqs: int, heads: int, group: int, rows: int, max_seqle
     if few_rows >= max_seqlen:
         return few_rows, few, 0
     tiles = heads * (rows * group // 128 + seqs)
-    return few_rows, few, max(1, min(-(-512 // tiles), -(-max_context // 512), 32))
+    most = max(1, min(-(-max_context // 512), 16)) if tiles < 1024 else 1
+    return few_rows, few, min(range(1, most + 1), key=lambda n: (-(-tiles * n // 512) + 0.1) / n + 0.01 * n)
 
 
 def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
