@@ -352,10 +352,12 @@ __device__ __forceinline__ u32x2_t codes_scaled(uint32_t c, f16x2_t f) {
   return r;
 }
 
-// A 64-key step's four tiles, in lanes: lane i holds tile i % 4.
+// A 64-key step's four tiles, in lanes: lane i holds tile i % 4.  As loaded, a
+// step or two before they are looked at: an id that is not checked yet is a
+// load that need not have come.
 struct StepTiles {
   int id;        // block, -1: no such block or past the keys
-  float sk, sv;  // its scales
+  float sk, sv;  // its scales, if there is one
 };
 __device__ __forceinline__ float quad_max(float v) {  // over the four tiles
   v = fmaxf(v, dpp_mov_f<0xB1>(v));
@@ -431,15 +433,16 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
   const int bmask = (1 << a.shift) - 1;
 
   const int quad16 = 16 * (lane & 3);
-  auto ids_of = [&](int gi) {
-    const int key = gi * kGroupKeys + quad16;
-    const int id = row_table[min(key, keys - 1) >> a.shift];
-    return gi < g1 && key < keys && id < a.num_blocks ? id : -1;
+  auto raw_ids = [&](int gi) { return row_table[min(gi * kGroupKeys + quad16, keys - 1) >> a.shift]; };
+  auto checked = [&](int gi, int id) {
+    return (gi < g1) & (gi * kGroupKeys + quad16 < keys) & (id < a.num_blocks) ? id : -1;
   };
-  auto scales_of = [&](int id) {
+  auto raw_scales = [&](int id) {
     const int64_t at = (int64_t)max(id, 0) * a.sc_b + h;
-    const float sk = a.k_scale[at], sv = a.v_scale[at];
-    return StepTiles{id, id < 0 ? 0.0f : sk, id < 0 ? 0.0f : sv};
+    return StepTiles{id, a.k_scale[at], a.v_scale[at]};
+  };
+  auto there_only = [&](StepTiles s) {
+    return StepTiles{s.id, s.id < 0 ? 0.0f : s.sk, s.id < 0 ? 0.0f : s.sv};
   };
   u32x4_t kr[KP], vr[KP];
   auto load_codes = [&](int gi, int ids) {
@@ -490,14 +493,17 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
     }
   };
   float ktop = 1.17549435e-38f, vtop = 1.17549435e-38f;  // of the keys in the buffer being read
-  StepTiles cur = {-1, 0.0f, 0.0f}, nxt = cur;
-  int ids2 = -1;  // of the step after next
+  StepTiles cur = {-1, 0.0f, 0.0f}, nxt = cur;  // of the step being read, and the next (scales not looked at)
+  int ids2 = -1;                                // of the step after that, not checked
   if (g0 < g1) {
-    const int ids0 = ids_of(g0), ids1 = ids_of(g0 + 1);
-    ids2 = ids_of(g0 + 2);
-    cur = scales_of(ids0);
-    nxt = scales_of(ids1);
+    int ids0 = raw_ids(g0), ids1 = raw_ids(g0 + 1);
+    ids2 = raw_ids(g0 + 2);
+    ids0 = checked(g0, ids0);
+    ids1 = checked(g0 + 1, ids1);
+    cur = raw_scales(ids0);
+    nxt = raw_scales(ids1);
     load_codes(g0, ids0);
+    cur = there_only(cur);
     ktop = fmaxf(ktop, quad_max(cur.sk));
     vtop = fmaxf(vtop, quad_max(cur.sv));
     write_codes(g0, 0, cur, ktop, vtop);
@@ -533,13 +539,14 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
     float ktop_n = ktop, vtop_n = vtop;
     const unsigned there = (unsigned)__ballot(cur.id >= 0) & 15u;
     if (gi + 1 < g1) {
-      ktop_n = fmaxf(ktop, quad_max(nxt.sk));
-      vtop_n = fmaxf(vtop, quad_max(nxt.sv));
-      write_codes(gi + 1, buf ^ 1, nxt, ktop_n, vtop_n);
-      cur = nxt;
-      nxt = scales_of(ids2);
+      cur = there_only(nxt);
+      ktop_n = fmaxf(ktop, quad_max(cur.sk));
+      vtop_n = fmaxf(vtop, quad_max(cur.sv));
+      write_codes(gi + 1, buf ^ 1, cur, ktop_n, vtop_n);
+      ids2 = checked(gi + 2, ids2);
+      nxt = raw_scales(ids2);
       load_codes(gi + 2, ids2);
-      ids2 = ids_of(gi + 3);
+      ids2 = raw_ids(gi + 3);
     }
     if (busy) {
       if (there != 15u || key0 + kGroupKeys > wfull) {
