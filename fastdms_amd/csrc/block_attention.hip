@@ -16,6 +16,8 @@
 // group g ends up with the 16 tokens of tile g in registers, and that is what
 // the second product wants of it: no shuffle and no LDS between the two, and K
 // and V go from memory straight to the operand registers.
+#include <type_traits>
+
 #include "fdms_block_kv.h"
 
 namespace fdms {
@@ -310,26 +312,32 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
   }
 }
 
-// Sequences of many query rows: 128 rows of a kv head (128 / group tokens, all
-// of the group's heads) per workgroup, 32 per wave, over one split of the keys.
+// Sequences of many query rows: 32 rows of a kv head (32 / group tokens, all of
+// the group's heads) per wave over one split of the keys, NW waves a workgroup.
 //
 // 64 keys at a time go from the cache to LDS as halves, converted once by the
-// workgroup's four waves (wave w tile w) and read by each of them; two buffers,
-// one barrier per 64 keys, the codes of the next keys but one on their way in
-// registers meanwhile.  v_mfma_f32_32x32x16_f16 with S^T = K Q^T, O^T = V^T P^T:
+// workgroup's waves and read by each of them; two buffers each of K and V, one
+// barrier per 64 keys.  v_mfma_f32_32x32x16_f16 with S^T = K Q^T, O^T = V^T P^T:
 // a lane owns one query (column lane % 32).  V's 16 tokens are written in the
 // order in which a lane of a score tile holds them (0-3, 8-11, 4-7, 12-15), so
 // P goes from one product to the other in registers.
 //
+// The matrix cores and the vector unit are about equally loaded (the
+// exponentials, and the conversion of the codes), so they have to run at the
+// same time: step t's exponentials stand beside the product of step t + 1's
+// keys, the conversion of step t + 2's K and t + 1's V beside step t's P V.  The
+// codes come from memory one step before they are converted, block ids one step
+// before those.
+//
 // The blocks' scales go into the halves: a block's codes times its scale over
 // the largest so far (a power of two no greater than 1 for the store's scales).
-// What falls below a half's range there is 2^-25 of that largest scale, far less than the fp32
-// sum it joins can hold next to it.  Then one factor holds for all keys of a
-// step, and exp(s - max) is one fma and one v_exp_f32 per score.
+// What falls below a half's range there is 2^-25 of that largest scale, far less
+// than the fp32 sum it joins can hold next to it.  Then one factor holds for all
+// keys of a step, and exp(s - max) is one fma and one v_exp_f32 per score.
 //
 // A row's maximum is raised only when a score passes it by 2^8 (P stays below
 // 2^8, in a half's range): O is rescaled in the first steps and hardly again.
-constexpr int kTileRows = 128;
+constexpr int kTileWaves = 4, kTileRows = 32 * kTileWaves;
 constexpr float kLazyMax = 8.0f;
 
 __device__ __forceinline__ float half_max(float v) {  // over lanes l, l ^ 32
@@ -352,36 +360,46 @@ __device__ __forceinline__ u32x2_t codes_scaled(uint32_t c, f16x2_t f) {
   return r;
 }
 
-// A 64-key step's four tiles, in lanes: lane i holds tile i % 4.  As loaded, a
-// step or two before they are looked at: an id that is not checked yet is a
-// load that need not have come.
-struct StepTiles {
-  int id;        // block, -1: no such block or past the keys
-  float sk, sv;  // its scales, if there is one
-};
-__device__ __forceinline__ float quad_max(float v) {  // over the four tiles
+__device__ __forceinline__ float quad_max(float v) {  // over the four tiles, the same for the wave (a scalar register)
   v = fmaxf(v, dpp_mov_f<0xB1>(v));
-  return fmaxf(v, dpp_mov_f<0x4E>(v));
+  v = fmaxf(v, dpp_mov_f<0x4E>(v));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
+// The larger of two scalars that are not negative (or NaN), whose bits order as they do: stays in scalar registers.
+__device__ __forceinline__ float scalar_max(float a, float b) {
+  return __builtin_bit_cast(float, max(__builtin_bit_cast(int, a), __builtin_bit_cast(int, b)));
+}
+
+// 16-byte chunk c of row r of a K step (2 D bytes a row) or V step (128 bytes)
+// lies at slot c ^ swizzle(r): 16 rows' chunks c spread over the 64 LDS banks.
+template <int BYTES>
+__device__ __forceinline__ int lds_swizzle(int row) {
+  return BYTES == 256 ? row & 15 : (row >> 1) & 7;
 }
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttnArgs a, int splits) {
-  constexpr int KSTEP = D / 16, DT = D / 32, KP = D / 64;
-  __shared__ u32x4_t s_k[2][64 * D / 8];  // 16-byte chunks, chunk c of row r at c ^ (r & 7)
-  __shared__ u32x4_t s_v[2][64 * D / 8];
+__global__ __launch_bounds__(64 * kTileWaves, 2) void block_attn_tile_kernel(const BlockAttnArgs a, int splits) {
+  constexpr int KSTEP = D / 16, DT = D / 32, KP = D / 64, ROWS = kTileRows;
+  constexpr int KB = 64 * D * 2;          // bytes of a step's K or V in LDS
+  __shared__ __align__(16) uint8_t s_kv[4 * KB];  // K, K, V, V
   const int pairs = a.num_seqs * a.num_kv_heads;
   const int pair = blockIdx.x % pairs, split = blockIdx.x / pairs;
-  const int b = pair / a.num_kv_heads, h = pair % a.num_kv_heads;
+  // Consecutive workgroups go to the XCDs in turn, and on an XCD to its shader
+  // engines in turn: the head stays the fastest index (a head's tiles share
+  // its K and V in one L2), and the sequence turns with the tile, or one engine
+  // would get all tiles of the longest sequence.
+  const int b = (int)((pair / a.num_kv_heads + blockIdx.y) % (unsigned)a.num_seqs), h = pair % a.num_kv_heads;
   const SeqSpan sp = seq_span(a, b);
   if (sp.n <= a.few_rows) return;
-  const int rows = sp.n * a.group, tiles = (rows + kTileRows - 1) / kTileRows;
+  const int rows = sp.n * a.group, tiles = (rows + ROWS - 1) / ROWS;
   const int tile = tiles - 1 - (int)blockIdx.y;  // the tiles that see most keys first
   if (tile < 0) return;
-  const int row0 = tile * kTileRows;
+  const int row0 = tile * ROWS;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int first_vis = sp.ctx - sp.n + 1;  // keys query 0 sees
-  const int keys = min(sp.ctx, first_vis + (min(row0 + kTileRows, rows) - 1) / a.group);  // that the tile sees
+  const int keys = min(sp.ctx, first_vis + (min(row0 + ROWS, rows) - 1) / a.group);  // that the tile sees
   const int groups = keys > 0 ? (keys + kGroupKeys - 1) / kGroupKeys : 0;
   const int used = splits_used(groups, splits, 8);
   if (split >= used) return;
@@ -391,15 +409,12 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
   // Q^T operand: channels 16 s + 8 half .. + 7 of row c
   const int r = row0 + wave * 32 + c;
   const bool on = r < rows;
-  const int t = sp.q0 + (on ? r / a.group : 0), head = h * a.group + (on ? r % a.group : 0);
   const int vis = on ? min(sp.ctx, first_vis + r / a.group) : 0;
-  // keys that all / any of the wave's rows see
-  const int wfull = first_vis + (row0 + wave * 32) / a.group;
-  const int wrows = min(rows - (row0 + wave * 32), 32);
-  const int wkeys = wrows > 0 ? min(sp.ctx, first_vis + (row0 + wave * 32 + wrows - 1) / a.group) : 0;
+  const int wfull = first_vis + (row0 + wave * 32) / a.group;  // keys that all of the wave's rows see
   f16x8_t qf[KSTEP];
   float qmul;
   {
+    const int t = sp.q0 + (on ? r / a.group : 0), head = h * a.group + (on ? r % a.group : 0);
     const int64_t at = (int64_t)t * a.qs_t + (int64_t)head * a.qs_h;
     u32x4_t raw[KSTEP];
 #pragma unroll
@@ -420,11 +435,9 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
       for (int j = 0; j < 8; ++j) qf[s][j] = (f16_t)(x[s][j] * qf_mul);
   }
 
-  f32x16_t o[DT];
+  f32x16_t o[DT], sa[2], sb[2];
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
+  for (int d = 0; d < DT; ++d) o[d] = f32x16_t{};
   float mx = kNegInf, l = 0.0f;
 
   const int32_t* row_table = a.tables + (int64_t)b * a.bt_b;
@@ -432,205 +445,258 @@ __global__ __launch_bounds__(256, 2) void block_attn_tile_kernel(const BlockAttn
   const uint8_t* vbase = a.vc + (int64_t)h * a.vc_h;
   const int bmask = (1 << a.shift) - 1;
 
+  // A step's four tiles are looked up by lane: lane i holds tile i % 4.  Ids and
+  // scales are kept as loaded until the step that needs them: looking at one
+  // earlier would wait for its load.
   const int quad16 = 16 * (lane & 3);
   auto raw_ids = [&](int gi) { return row_table[min(gi * kGroupKeys + quad16, keys - 1) >> a.shift]; };
-  auto checked = [&](int gi, int id) {
-    return (gi < g1) & (gi * kGroupKeys + quad16 < keys) & (id < a.num_blocks) ? id : -1;
+  auto checked = [&](int gi, int id) {  // -1: no such block, or past the keys
+    return ((gi < g1) & (gi * kGroupKeys + quad16 < keys) & (id < a.num_blocks)) ? id : -1;
   };
-  auto raw_scales = [&](int id) {
-    const int64_t at = (int64_t)max(id, 0) * a.sc_b + h;
-    return StepTiles{id, a.k_scale[at], a.v_scale[at]};
-  };
-  auto there_only = [&](StepTiles s) {
-    return StepTiles{s.id, s.id < 0 ? 0.0f : s.sk, s.id < 0 ? 0.0f : s.sv};
-  };
-  u32x4_t kr[KP], vr[KP];
-  auto load_codes = [&](int gi, int ids) {
+  auto scale_of = [&](const float* scales, int id) { return scales[(int64_t)max(id, 0) * a.sc_b + h]; };
+  auto load_codes = [&](u32x4_t* raw, const uint8_t* base, int64_t stride, int gi, int ids) {
     const int id = max(__builtin_amdgcn_readlane(ids, wave), 0);
-    const int in_block = (gi * kGroupKeys + 16 * wave) & bmask;
-    const uint8_t* kp = kbase + (int64_t)id * a.kc_b + in_block * D + lane * 16;
-    const uint8_t* vp = vbase + (int64_t)id * a.vc_b + in_block * D + lane * 16;
+    const uint8_t* p = base + (int64_t)id * stride + ((gi * kGroupKeys + 16 * wave) & bmask) * D + lane * 16;
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
-      kr[p] = *(const u32x4_t*)(kp + 1024 * p);
-      vr[p] = *(const u32x4_t*)(vp + 1024 * p);
+    for (int i = 0; i < KP; ++i) raw[i] = *(const u32x4_t*)(p + 1024 * i);
+  };
+  // the factor of the wave's tile: its scale over the largest so far
+  auto factor = [&](float scale, float top) {
+    const float s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), wave));
+    const f16_t f = (f16_t)(s * __builtin_amdgcn_rcpf(top));
+    return f16x2_t{f, f};
+  };
+  // Where the lane's first piece goes: chunk 2 p of its row, and 2 p + 1 at ^ 16
+  // (the second piece: eight K rows or 64 V rows on, at the same p).
+  const uint32_t kw0 = (16 * wave + lane / (D / 16)) * (2 * D) +
+                       (((2 * (lane % (D / 16))) ^ lds_swizzle<2 * D>(16 * wave + lane / (D / 16))) << 4);
+  const uint32_t vw0 = 2 * KB + lane * 128 + (((2 * wave) ^ lds_swizzle<128>(lane)) << 4);
+  auto kw = [&](int i) { return i ? (kw0 + 8 * 2 * D) ^ (8u << 4) : kw0; };
+  auto vw = [&](int i) { return vw0 + i * 64 * 128; };
+  // One of the 4 KP words of the wave's codes, to halves in w; each second word completes a 16-byte chunk.
+  auto convert_k = [&](const u32x4_t* raw, int n, int buf, f16x2_t f, u32x4_t& w) {
+    const int i = n >> 2, j = n & 3;
+    const u32x2_t x = codes_scaled<FP8>(raw[i][j], f);
+    w[2 * (j & 1)] = x[0];
+    w[2 * (j & 1) + 1] = x[1];
+    if (j & 1) *(u32x4_t*)(s_kv + ((kw(i) ^ (16u * (j >> 1))) + buf * KB)) = w;
+  };
+  auto convert_v = [&](const u32x4_t* raw, int n, int buf, f16x2_t f, u32x4_t& w) {
+    const int i = n >> 2, j = n & 3;  // words 0, 2, then 1, 3
+    const u32x2_t x = codes_scaled<FP8>(raw[i][(j >> 1) | ((j & 1) << 1)], f);
+    w[2 * (j & 1)] = x[0];
+    w[2 * (j & 1) + 1] = x[1];
+    if (j & 1) *(u32x4_t*)(s_kv + ((vw(i) ^ (16u * (j >> 1))) + buf * KB)) = w;
+  };
+  auto drop_past_keys = [&](u32x4_t* raw, int gi, int ids) {
+    if constexpr (FP8) {  // V's tokens past the keys may hold NaN codes, and 0 * NaN is no 0
+      const int live = __builtin_amdgcn_readlane(ids, wave) < 0 ? 0 : keys - (gi * kGroupKeys + 16 * wave);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nb = min(max(live - 4 * j, 0), 4);
+        const uint32_t keep = (uint32_t)((1ull << (8 * nb)) - 1);
+#pragma unroll
+        for (int i = 0; i < KP; ++i) raw[i][j] &= keep;
+      }
     }
   };
-  // the wave's tile to LDS; ktop / vtop: the largest scales so far
-  auto write_codes = [&](int gi, int buf, const StepTiles& s, float ktop, float vtop) {
-    const float sk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s.sk), wave));
-    const float sv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s.sv), wave));
-    const int id = __builtin_amdgcn_readlane(s.id, wave);
-    const f16_t fk = (f16_t)(sk * __builtin_amdgcn_rcpf(ktop)), fv = (f16_t)(sv * __builtin_amdgcn_rcpf(vtop));
-    const f16x2_t fk2 = {fk, fk}, fv2 = {fv, fv};
-    const int live = id < 0 ? 0 : keys - (gi * kGroupKeys + 16 * wave);
+  // the lane's first operand chunks; those of channel step s and of 16 keys u are at ^ 32 s and ^ 32 u
+  const uint32_t ka0 = c * (2 * D) + ((half ^ lds_swizzle<2 * D>(c)) << 4);
+  const uint32_t va0 = 2 * KB + c * 128 + ((half ^ lds_swizzle<128>(c)) << 4);
+
+  auto mask = [&](f32x16_t(&sx)[2], int gi, unsigned there) {
+    const int rel = vis - gi * kGroupKeys - 4 * half;  // keys the row sees of the step, less the lane's first
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
-      const int at = lane + 64 * p, row = 16 * wave + at / (D / 16), chunk = 2 * (at % (D / 16));
-      u32x4_t w0, w1;
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x2_t x = codes_scaled<FP8>(kr[p][j], fk2), y = codes_scaled<FP8>(kr[p][2 + j], fk2);
-        w0[2 * j] = x[0], w0[2 * j + 1] = x[1], w1[2 * j] = y[0], w1[2 * j + 1] = y[1];
+      for (int j = 0; j < 16; ++j) {
+        const int lim = (there >> (2 * x + (j >> 3))) & 1 ? rel : -64;
+        sx[x][j] = 32 * x + 8 * (j >> 2) + (j & 3) >= lim ? kNegInf : sx[x][j];
       }
-      s_k[buf][row * (D / 8) + (chunk ^ (row & 7))] = w0;
-      s_k[buf][row * (D / 8) + ((chunk + 1) ^ (row & 7))] = w1;
-      // V: channel at of the tile; tokens past the keys may hold NaN codes, and 0 * NaN is no 0
-      if (live < kTile) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int nb = min(max(live - 4 * j, 0), 4);
-          vr[p][j] &= nb == 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x2_t x = codes_scaled<FP8>(vr[p][2 * j], fv2), y = codes_scaled<FP8>(vr[p][2 * j + 1], fv2);
-        w0[2 * j] = x[0], w0[2 * j + 1] = x[1], w1[2 * j] = y[0], w1[2 * j + 1] = y[1];
-      }
-      s_v[buf][at * 8 + ((2 * wave) ^ (at & 7))] = w0;
-      s_v[buf][at * 8 + ((2 * wave + 1) ^ (at & 7))] = w1;
-    }
   };
-  float ktop = 1.17549435e-38f, vtop = 1.17549435e-38f;  // of the keys in the buffer being read
-  StepTiles cur = {-1, 0.0f, 0.0f}, nxt = cur;  // of the step being read, and the next (scales not looked at)
-  int ids2 = -1;                                // of the step after that, not checked
-  if (g0 < g1) {
-    int ids0 = raw_ids(g0), ids1 = raw_ids(g0 + 1);
-    ids2 = raw_ids(g0 + 2);
-    ids0 = checked(g0, ids0);
-    ids1 = checked(g0 + 1, ids1);
-    cur = raw_scales(ids0);
-    nxt = raw_scales(ids1);
-    load_codes(g0, ids0);
-    cur = there_only(cur);
-    ktop = fmaxf(ktop, quad_max(cur.sk));
-    vtop = fmaxf(vtop, quad_max(cur.sv));
-    write_codes(g0, 0, cur, ktop, vtop);
-    load_codes(g0 + 1, ids1);
-  }
-  __syncthreads();
-  for (int gi = g0; gi < g1; ++gi) {
-    const int buf = (gi - g0) & 1, key0 = gi * kGroupKeys;
-    const bool busy = key0 < wkeys;
-    f32x16_t st[2];
-    if (busy) {
-      for (int x = 0; x < 2; ++x)
+  auto row_max = [&](const f32x16_t(&sx)[2]) {
+    float m0 = kNegInf, m1 = kNegInf;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) st[x][j] = 0.0f;
-#pragma unroll
-      for (int s0 = 0; s0 < KSTEP; s0 += 4) {  // eight operands on their way at once
-        f16x8_t kf[4][2];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            kf[s][x] = __builtin_bit_cast(
-                f16x8_t, s_k[buf][(32 * x + c) * (D / 8) + ((2 * (s0 + s) + half) ^ (c & 7))]);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            st[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s][x], qf[s0 + s], st[x], 0, 0, 0);
-      }
+    for (int j = 0; j < 16; ++j) {
+      m0 = fmaxf(fmaxf(m0, sx[0][j]), sx[1][j]);
+      ++j;
+      m1 = fmaxf(fmaxf(m1, sx[0][j]), sx[1][j]);
     }
-    // the next keys into the other buffer, those after them on their way
-    float ktop_n = ktop, vtop_n = vtop;
-    const unsigned there = (unsigned)__ballot(cur.id >= 0) & 15u;
-    if (gi + 1 < g1) {
-      cur = there_only(nxt);
-      ktop_n = fmaxf(ktop, quad_max(cur.sk));
-      vtop_n = fmaxf(vtop, quad_max(cur.sv));
-      write_codes(gi + 1, buf ^ 1, cur, ktop_n, vtop_n);
-      ids2 = checked(gi + 2, ids2);
-      nxt = raw_scales(ids2);
-      load_codes(gi + 2, ids2);
-      ids2 = raw_ids(gi + 3);
+    return fmaxf(m0, m1);
+  };
+  // the running maximum takes in a step's scores (times mul); exp2(fma(score, mul, -base)) are then its weights
+  float mul = 0.0f, base = 0.0f;
+  auto raise = [&](f32x16_t(&sx)[2], float lane_max, float top_scale) {
+    mul = fmaxf(qmul * top_scale, 1e-37f);  // above 0: -inf stays -inf
+    const float top = half_max(lane_max) * mul;
+    if (__any(top > mx + kLazyMax)) {
+      const float mnew = fmaxf(mx, top);
+      const float alpha = __builtin_amdgcn_exp2f(mx - (mnew == kNegInf ? 0.0f : mnew));
+      mx = mnew;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
     }
-    if (busy) {
-      if (there != 15u || key0 + kGroupKeys > wfull) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int key = 32 * x + 8 * (j >> 2) + 4 * half + (j & 3);
-            if (key0 + key >= vis || !((there >> (2 * x + (j >> 3))) & 1)) st[x][j] = kNegInf;
-          }
-      }
-      const float mul = fmaxf(qmul * ktop, 1e-37f);  // above 0: -inf stays -inf
-      float top = kNegInf;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, st[x][j]);
-      top = half_max(top) * mul;
-      if (__any(top > mx + kLazyMax)) {
-        const float mnew = fmaxf(mx, top);
-        const float alpha = __builtin_amdgcn_exp2f(mx - (mnew == kNegInf ? 0.0f : mnew));
-        mx = mnew;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= alpha;
-      }
-      const float base = mx == kNegInf ? 0.0f : mx;
-      // scores so large that the product's rounding, which base has and the fma has not, would show
-      if (__any(fabsf(base) > 65536.0f)) {
+    base = mx == kNegInf ? 0.0f : mx;
+    // scores so large that the product's rounding, which mx has and the fma has not, would show
+    if (__builtin_expect(__any(fabsf(base) > 65536.0f), 0)) {
 #pragma clang fp contract(off)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float prod = st[x][j] * mul;
-            st[x][j] = prod - base;
-          }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) st[x][j] = __builtin_fmaf(st[x][j], mul, -base);
-      }
-      f16x8_t pf[4], vf[2][4];
-      auto load_v = [&](int d) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          vf[d & 1][u] = __builtin_bit_cast(f16x8_t, s_v[buf][(32 * d + c) * 8 + ((2 * u + half) ^ (c & 7))]);
-      };
-      load_v(0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          f32x2_t p;
-          p[0] = __builtin_amdgcn_exp2f(st[x][j]);
-          p[1] = __builtin_amdgcn_exp2f(st[x][j + 1]);
-          const f16x2_t ph = __builtin_convertvector(p, f16x2_t);
-          const f16x2_t one = {(f16_t)1.0f, (f16_t)1.0f};
-          l = __builtin_amdgcn_fdot2(ph, one, l, false);
-          pf[2 * x + (j >> 3)][j & 7] = ph[0];
-          pf[2 * x + (j >> 3)][(j & 7) + 1] = ph[1];
+        for (int j = 0; j < 16; ++j) {
+          const float prod = sx[x][j] * mul;
+          sx[x][j] = prod - base;
         }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        if (d + 1 < DT) load_v(d + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d & 1][u], pf[u], o[d], 0, 0, 0);
-      }
+      mul = 1.0f;
+      base = 0.0f;
     }
-    if (vtop_n > vtop) {
-      const float f = vtop * __builtin_amdgcn_rcpf(vtop_n);
+  };
+  // weights n and n + 1 of the lane's 32, as halves and in the row's sum
+  auto weigh = [&](const f32x16_t(&sx)[2], int n, f16x8_t(&pf)[4]) {
+    const int x = n >> 4, j = n & 15;
+    f32x2_t p;
+    p[0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[x][j], mul, -base));
+    p[1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[x][j + 1], mul, -base));
+    const f16x2_t ph = __builtin_convertvector(p, f16x2_t), one = {(f16_t)1.0f, (f16_t)1.0f};
+    l = __builtin_amdgcn_fdot2(ph, one, l, false);
+    pf[n >> 3][n & 7] = ph[0];
+    pf[n >> 3][(n & 7) + 1] = ph[1];
+  };
+  // operand i of a step's products: K's (channel step i / 2, key half i % 2), then V's (16 keys u, channels 32 d)
+  auto operand = [&](int i, int kbuf, int vbuf) {
+    const int n = i - 2 * KSTEP;
+    const uint32_t at = i < 2 * KSTEP ? kbuf * KB + (i & 1) * (64 * D) + (ka0 ^ (32u * (i >> 1)))
+                                      : vbuf * KB + (n % DT) * 4096 + (va0 ^ (32u * (n / DT)));
+    return *(const f16x8_t*)(s_kv + at);
+  };
+
+  // State at step gi (buffer B = parity): cur its masked scores; kr / vr the codes of K(gi + 2) and V(gi + 1), idk / idv and skr / svr
+  // their blocks and scales as loaded; ids3 the ids of gi + 3, not checked.
+  u32x4_t kr[KP], vr[KP];
+  float ktop = 1.17549435e-38f, vtop = 1.17549435e-38f;  // largest scales of K(gi + 1), V(gi)
+  float skr = 0.0f, svr = 0.0f;
+  int idk = -1, idv = -1, ids3 = -1;
+  auto there_only = [&](float s, int id) { return id < 0 ? 0.0f : s; };
+  if (g0 < g1) {
+    const int i0 = raw_ids(g0), i1 = raw_ids(g0 + 1), i2 = raw_ids(g0 + 2);
+    ids3 = raw_ids(g0 + 3);
+    const int id0 = checked(g0, i0), id1 = checked(g0 + 1, i1);
+    idk = checked(g0 + 2, i2);
+    idv = id1;
+    u32x4_t k0[KP], k1[KP], v0[KP];
+    load_codes(k0, kbase, a.kc_b, g0, id0);
+    load_codes(v0, vbase, a.vc_b, g0, id0);
+    load_codes(k1, kbase, a.kc_b, g0 + 1, id1);
+    const float sk0 = there_only(scale_of(a.k_scale, id0), id0), sk1 = there_only(scale_of(a.k_scale, id1), id1);
+    const float sv0 = there_only(scale_of(a.v_scale, id0), id0);
+    load_codes(kr, kbase, a.kc_b, g0 + 2, idk);
+    load_codes(vr, vbase, a.vc_b, g0 + 1, idv);
+    skr = scale_of(a.k_scale, idk);
+    svr = scale_of(a.v_scale, idv);
+    const float ktop0 = scalar_max(ktop, quad_max(sk0));
+    ktop = scalar_max(ktop0, quad_max(sk1));
+    vtop = scalar_max(vtop, quad_max(sv0));
+    drop_past_keys(v0, g0, id0);
+    const f16x2_t fk0 = factor(sk0, ktop0), fk1 = factor(sk1, ktop), fv0 = factor(sv0, vtop);
+    u32x4_t w0, w1, w2;
+#pragma unroll
+    for (int n = 0; n < 4 * KP; ++n) {
+      convert_k(k0, n, 0, fk0, w0);
+      convert_k(k1, n, 1, fk1, w1);
+      convert_v(v0, n, 0, fv0, w2);
+    }
+    __syncthreads();
+    sa[0] = sa[1] = f32x16_t{};
+#pragma unroll
+    for (int i = 0; i < 2 * KSTEP; ++i)
+      sa[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand(i, 0, 0), qf[i >> 1], sa[i & 1], 0, 0, 0);
+    const unsigned there = (unsigned)__ballot(id0 >= 0) & 15u;
+    if (there != 15u || (g0 + 1) * kGroupKeys > wfull) mask(sa, g0, there);
+    raise(sa, row_max(sa), ktop0);
+  }
+  __syncthreads();  // K(g0) has been read: its buffer takes K(g0 + 2)
+  auto step = [&](int gi, auto parity, f32x16_t(&cur)[2], f32x16_t(&nxt)[2]) {
+    constexpr int B = decltype(parity)::value;
+    // In this order, which the compiler left to itself does not find: operands
+    // read AHEAD products before theirs, between the products of the first half
+    // the exponentials, between those of the second the codes and the maximum.
+    constexpr int NK = 2 * KSTEP, N = NK + 4 * DT, AHEAD = D == 128 ? 2 : 4;
+    f16x8_t pf[4], fr[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fr[i] = operand(i, 1 - B, B);
+    nxt[0] = nxt[1] = f32x16_t{};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      nxt[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[i % AHEAD], qf[i >> 1], nxt[i & 1], 0, 0, 0);
+      fr[i % AHEAD] = operand(i + AHEAD, 1 - B, B);
+#pragma unroll
+      for (int n = 0; n < 32 / NK; n += 2) weigh(cur, i * (32 / NK) + n, pf);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // K(gi + 2) and V(gi + 1) go into the buffers that step gi - 1 read
+    const float sk = there_only(skr, idk), sv = there_only(svr, idv);
+    const float ktop2 = scalar_max(ktop, quad_max(sk)), vtop1 = scalar_max(vtop, quad_max(sv));
+    const f16x2_t fk = factor(sk, ktop2), fv = factor(sv, vtop1);
+    const unsigned there = (unsigned)__ballot(idv >= 0) & 15u;  // of step gi + 1
+    drop_past_keys(vr, gi + 1, idv);
+    u32x4_t wk, wv;
+    float m0 = kNegInf, m1 = kNegInf;
+#pragma unroll
+    for (int i = 0; i < N - NK; ++i) {
+      const int d = i % DT, u = i / DT;
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr[(NK + i) % AHEAD], pf[u], o[d], 0, 0, 0);
+      if (NK + i + AHEAD < N) fr[(NK + i) % AHEAD] = operand(NK + i + AHEAD, 1 - B, B);
+      constexpr int UNITS = 8 * KP / (N - NK);  // 8 KP words of codes over 4 DT products
+      static_assert(UNITS == 1, "one word per product");
+      if (i < 4 * KP) convert_k(kr, i, B, fk, wk);
+      else convert_v(vr, i - 4 * KP, 1 - B, fv, wv);
+#pragma unroll
+      for (int n = 0; n < 16 / (N - NK); ++n) {
+        const int j = i * (16 / (N - NK)) + n;
+        float& m = j & 1 ? m1 : m0;
+        m = fmaxf(fmaxf(m, nxt[0][j]), nxt[1][j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    idv = idk;
+    idk = checked(gi + 3, ids3);
+    load_codes(kr, kbase, a.kc_b, gi + 3, idk);
+    load_codes(vr, vbase, a.vc_b, gi + 2, idv);
+    skr = scale_of(a.k_scale, idk);
+    svr = scale_of(a.v_scale, idv);
+    ids3 = raw_ids(gi + 4);
+    float lane_max = fmaxf(m0, m1);
+    if (there != 15u || (gi + 2) * kGroupKeys > wfull) {
+      mask(nxt, gi + 1, there);
+      lane_max = row_max(nxt);
+    }
+    raise(nxt, lane_max, ktop);
+    if (vtop1 > vtop) {
+      const float f = vtop * __builtin_amdgcn_rcpf(vtop1);
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
     }
-    ktop = ktop_n;
-    vtop = vtop_n;
+    ktop = ktop2;
+    vtop = vtop1;
     __syncthreads();
+  };
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+  for (int gi = g0; gi < g1; gi += 2) {
+    step(gi, even, sa, sb);
+    if (gi + 1 < g1) step(gi + 1, odd, sb, sa);
   }
 
   const float sum = half_sum(l);
-  if (!on) return;
+  // the lane's row again, from a thread id the compiler cannot tell is the same: held over the loop it
+  // would cost registers there
+  int tid_out = threadIdx.x;
+  asm volatile("" : "+v"(tid_out));
+  const int r_out = row0 + (tid_out >> 6) * 32 + (tid_out & 31);
+  if (r_out >= rows) return;
+  const int t = sp.q0 + r_out / a.group, head = h * a.group + r_out % a.group;
   const float inv = used > 1 ? vtop : (sum == 0.0f ? 0.0f : vtop / sum);  // a row that sees no key: zeros
   const int64_t at = part_row(a, split, t, head);
 #pragma unroll
@@ -693,7 +759,7 @@ static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, in
   }
   if (tile_splits) {
     const dim3 grid((unsigned)(pairs * tile_splits), (unsigned)((max_rows - 1) / kTileRows + 1));
-    block_attn_tile_kernel<D, FP8><<<grid, 256, 0, st>>>(a, tile_splits);
+    block_attn_tile_kernel<D, FP8><<<grid, 64 * kTileWaves, 0, st>>>(a, tile_splits);
     FDMS_LAUNCH_CHECK();
   }
   const int splits = few_splits > tile_splits ? few_splits : tile_splits;
