@@ -72,7 +72,7 @@ SIGNATURES: dict[str, str] = {
     "fdms_block_tables": "ppiplipipiippppppp",
     "fdms_store_block_kvcache": "ppillllppillllpplpiiiiip",
     "fdms_gather_block_kvcache": "ppillllpplpiiiiippillllp",
-    "fdms_block_attention": "pillippillllpplplipppllpiiiiiiiiiifp",
+    "fdms_block_attention": "pillippillllpplplipppllpiiiiiiiiiiifp",
 }
 
 _CT = {"p": _P, "i": _I, "l": _L, "f": _F}

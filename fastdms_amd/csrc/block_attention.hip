@@ -23,6 +23,7 @@
 namespace fdms {
 
 constexpr int kGroupKeys = 64;  // keys a wave takes at once: four tiles
+constexpr int kMaxSplits = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -63,10 +64,11 @@ __device__ __forceinline__ SeqSpan seq_span(const BlockAttnArgs& a, int b) {
   return s;
 }
 
-// The splits a query tile uses of the launch's: of at least `least` 64-key
-// groups each, so a short context leaves the rest of its workgroups idle.
-__device__ __forceinline__ int splits_used(int groups, int splits, int least) {
-  return min(splits, max(1, groups / least));
+// The splits a query tile uses of the launch's: of about `share` 64-key groups
+// each, so a short context leaves the rest of its workgroups idle and a batch of
+// unequal ones is cut into equal pieces.
+__device__ __forceinline__ int splits_used(int groups, int splits, int share) {
+  return min(splits, max(1, (groups + share - 1) / share));
 }
 
 // Where a split's part of (row t of q, head) lies, in rows of D (part_o) or 2 (part_ml).
@@ -104,8 +106,12 @@ __device__ __forceinline__ float q_factor(float amax) {
 // Sequences of few query rows (row r: token r / group, head r % group of the kv
 // head; at most 16 * MT).  One workgroup takes all of them over one split of
 // the keys; its four waves take 64-key groups in turn and join at the end.
+// (three or four waves per SIMD with 16 rows, two with 32)
+template <int D, int MT>
+constexpr int kFewWaves = MT == 1 ? (D == 64 ? 4 : 3) : 2;
+
 template <int D, bool FP8, int MT>
-__global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, int splits) {
+__global__ __launch_bounds__(256, (kFewWaves<D, MT>)) void block_attn_kernel(const BlockAttnArgs a, int splits, int share) {
   constexpr int KL = D / 64, DC = D / 16, KS = D / 32;  // K loads per row and lane, V row groups, K steps
   constexpr int ROWS = 16 * MT, PAD = D + 4;
   __shared__ float s_o[4][ROWS][PAD];
@@ -120,7 +126,7 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
   const int first_vis = sp.ctx - sp.n + 1;  // keys query 0 sees
   const int keys = sp.ctx, full = first_vis;  // keys that the last query sees, and that all of them see
   const int groups = (keys + kGroupKeys - 1) / kGroupKeys;
-  const int used = splits_used(groups, splits, 4);
+  const int used = splits_used(groups, splits, share);
   if (split >= used) return;
   const int per = (groups + used - 1) / used;
   const int g_end = min(groups, (split + 1) * per);
@@ -168,46 +174,52 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
   const uint8_t* vbase = a.vc + (int64_t)h * a.vc_h;
   const int bmask = (1 << a.shift) - 1;
 
-  for (int gi = split * per + wave; gi < g_end; gi += 4) {
-    const int key0 = gi * kGroupKeys;
-    // the lane's V tile (g) and the tile of its K rows (c / 4)
-    const int kv_v = key0 + 16 * g, kv_k = key0 + 16 * (c >> 2);
-    const int idv = kv_v < keys ? row_table[kv_v >> a.shift] : -1;
-    const int idk = kv_k < keys ? row_table[kv_k >> a.shift] : -1;
-    const bool okv = idv >= 0 && idv < a.num_blocks, okk = idk >= 0 && idk < a.num_blocks;
-    const uint8_t* kp = kbase + (int64_t)(okk ? idk : 0) * a.kc_b + ((kv_k & bmask) + (c & 3)) * D + g * 16;
-    const uint8_t* vp = vbase + (int64_t)(okv ? idv : 0) * a.vc_b + (kv_v & bmask) * D + c * kTile;
-    u32x4_t kr[4][KL], vr[DC];
+  // The lane's V tile is g, that of its K rows c / 4.  Ids are loaded a step
+  // ahead of codes and scales, and a step's K as soon as the score product has
+  // taken the last one's, its V after the second product: the registers that hold
+  // one step's codes have the next one's on their way.
+  auto id_at = [&](int gi, int quarter) {  // as loaded; a step past the end reads its last one's
+    const int key = min(gi, g_end - 1) * kGroupKeys + 16 * quarter;
+    return row_table[min(key, keys - 1) >> a.shift];
+  };
+  auto there = [&](int gi, int quarter, int id) { return gi * kGroupKeys + 16 * quarter < keys && id >= 0 && id < a.num_blocks; };
+  u32x4_t kr[4][KL], vr[DC];
+  auto load_k = [&](int gi, int id) {
+    const int row = ((gi * kGroupKeys + 16 * (c >> 2)) & bmask) + (c & 3);
+    const uint8_t* p = kbase + (int64_t)id * a.kc_b + row * D + g * 16;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int x = 0; x < KL; ++x) kr[t][x] = *(const u32x4_t*)(kp + 4 * t * D + 64 * x);
+      for (int x = 0; x < KL; ++x) kr[t][x] = *(const u32x4_t*)(p + 4 * t * D + 64 * x);
+  };
+  auto load_v = [&](int gi, int id) {
+    const uint8_t* p = vbase + (int64_t)id * a.vc_b + ((gi * kGroupKeys + 16 * g) & bmask) * D + c * kTile;
 #pragma unroll
-    for (int d = 0; d < DC; ++d) vr[d] = *(const u32x4_t*)(vp + 256 * d);
-    const int64_t sc = (int64_t)(okv ? idv : 0) * a.sc_b + h;
-    const float sk = okv ? a.k_scale[sc] : 0.0f, sv = okv ? a.v_scale[sc] : 0.0f;
-    const int live = okv ? keys - kv_v : 0;  // of the lane's tile; rows past it hold whatever the block held
-    if constexpr (FP8) {
-      // a byte of an unwritten row may be a NaN code, and 0 * NaN is no 0
-      if (__any(live < kTile)) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int nb = min(max(live - 4 * w, 0), 4);
-          const uint32_t keep = nb == 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
-#pragma unroll
-          for (int d = 0; d < DC; ++d) vr[d][w] &= keep;
-        }
-      }
-    }
-    const float sv_top = rows_max(sv);
-    float osc = 1.0f;
-    if (sv_top > sref) {
-      osc = sref / sv_top;
-      sref = sv_top;
-    }
-    const float vmul = sv / sref;
-    const bool masked = __any(!okv) || key0 + kGroupKeys > full;
-
+    for (int d = 0; d < DC; ++d) vr[d] = *(const u32x4_t*)(p + 256 * d);
+  };
+  const int gi0 = split * per + wave;
+  float sk_n = 0.0f, sv_n = 0.0f;
+  int idk_n = 0, idv_n = 0;
+  bool okv_n = false;
+  if (gi0 < g_end) {
+    const int ik = id_at(gi0, c >> 2), iv = id_at(gi0, g);
+    idk_n = id_at(gi0 + 4, c >> 2);
+    idv_n = id_at(gi0 + 4, g);
+    okv_n = there(gi0, g, iv);
+    const int id = okv_n ? iv : 0;
+    load_k(gi0, there(gi0, c >> 2, ik) ? ik : 0);
+    sk_n = a.k_scale[(int64_t)id * a.sc_b + h];
+    sv_n = a.v_scale[(int64_t)id * a.sc_b + h];
+    load_v(gi0, id);
+  }
+  for (int gi = gi0; gi < g_end; gi += 4) {
+    const int key0 = gi * kGroupKeys, kv_v = key0 + 16 * g;
+    const bool okv = okv_n;
+    const float sk = okv ? sk_n : 0.0f, sv = okv ? sv_n : 0.0f;
+    // the next step's blocks (the last step's own once more where there is none)
+    const int gn = min(gi + 4, g_end - 1);
+    okv_n = there(gn, g, idv_n);
+    const int idk = there(gn, c >> 2, idk_n) ? idk_n : 0, idv = okv_n ? idv_n : 0;
     f32x4_t st[MT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -220,7 +232,24 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
         for (int m = 0; m < MT; ++m)
           st[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[m][s], st[m][t], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);  // or all codes are converted, into registers of their own, first
     }
+    load_k(gn, idk);
+    sk_n = a.k_scale[(int64_t)idv * a.sc_b + h];
+    sv_n = a.v_scale[(int64_t)idv * a.sc_b + h];
+    idk_n = id_at(gi + 8, c >> 2);
+    idv_n = id_at(gi + 8, g);
+    __builtin_amdgcn_sched_barrier(0);
+    const int live = okv ? keys - kv_v : 0;  // of the lane's tile; rows past it hold whatever the block held
+    const float sv_top = rows_max(sv);
+    float osc = 1.0f;
+    if (sv_top > sref) {
+      osc = sref / sv_top;
+      sref = sv_top;
+    }
+    const float vmul = sv / sref;
+    const bool masked = __any(!okv) || key0 + kGroupKeys > full;
+
     f16x8_t pf[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -259,14 +288,29 @@ __global__ __launch_bounds__(256) void block_attn_kernel(const BlockAttnArgs a, 
 #pragma unroll
       for (int d = 0; d < DC; ++d) o[m][d] *= f;
     }
+    if constexpr (FP8) {
+      // a byte of an unwritten row may be a NaN code, and 0 * NaN is no 0
+      if (__any(live < kTile)) {
 #pragma unroll
-    for (int d = 0; d < DC; ++d)
+        for (int w = 0; w < 4; ++w) {
+          const int nb = min(max(live - 4 * w, 0), 4);
+          const uint32_t keep = nb == 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
+#pragma unroll
+          for (int d = 0; d < DC; ++d) vr[d][w] &= keep;
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DC; ++d) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const f16x8_t vf = codes8_to_f16<FP8>(vr[d][2 * u], vr[d][2 * u + 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[m][u], o[m][d], 0, 0, 0);
       }
+      if (d & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    load_v(gn, idv);
   }
 
   // join the four waves: every partial to the workgroup's maximum
@@ -401,7 +445,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void block_attn_tile_kernel(con
   const int first_vis = sp.ctx - sp.n + 1;  // keys query 0 sees
   const int keys = min(sp.ctx, first_vis + (min(row0 + ROWS, rows) - 1) / a.group);  // that the tile sees
   const int groups = keys > 0 ? (keys + kGroupKeys - 1) / kGroupKeys : 0;
-  const int used = splits_used(groups, splits, 8);
+  const int used = min(splits, max(1, groups / 8));
   if (split >= used) return;
   const int per = (groups + used - 1) / used;
   const int g0 = split * per, g1 = min(groups, g0 + per);
@@ -717,28 +761,59 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void block_attn_tile_kernel(con
   }
 }
 
-// Joins the splits of the rows that used several: D / 4 lanes per row.
-template <int D>
+// Joins the splits of the rows that used several: D / 4 lanes hold a split's
+// part.  Few rows of many splits (a decode step) get a workgroup each, which
+// takes 1024 / D splits at a time and meets in LDS, the parts' loads not waiting
+// for the maxima that weigh them; many rows of few splits (SIDE 1) D / 4 lanes
+// each, one split after another.
+template <int D, int SIDE>
 __global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArgs a, int splits) {
-  constexpr int LPR = D / 4, RPG = 256 / LPR;
-  const int heads = a.num_kv_heads * a.group;
-  const int64_t row = (int64_t)blockIdx.x * RPG + threadIdx.x / LPR;
-  const int d = (threadIdx.x % LPR) * 4;
+  constexpr int LPR = D / 4, ROWS = 256 / (LPR * SIDE);
+  static_assert(SIDE == 1 || ROWS == 1, "a row per workgroup, or D / 4 lanes a row");
+  __shared__ f32x4_t s_v[SIDE][LPR];
+  __shared__ float s_f[kMaxSplits];
+  const int heads = a.num_kv_heads * a.group, tid = threadIdx.x;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + (SIDE == 1 ? tid / LPR : 0);
   const int t = (int)(row / heads), head = (int)(row % heads);
   if (t >= a.total_rows) return;
   if (a.cu && (t < a.cu[0] || t >= a.cu[a.num_seqs])) return;  // no sequence's row
   const int used = min(a.part_used[row], splits);
   if (used <= 1) return;
-  float top = kNegInf;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * part_row(a, s, t, head)]);
-  const float base = top == kNegInf ? 0.0f : top;
-  float sum = 0.0f;
-  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < used; ++s) {
-    const int64_t p = part_row(a, s, t, head);
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - base);
-    sum += a.part_ml[2 * p + 1] * f;
-    v += *(const f32x4_t*)(a.part_o + p * D + d) * f;
+  const int lane = tid & 63, side = SIDE == 1 ? 0 : tid / LPR, d = (tid % LPR) * 4;
+  const f32x4_t none = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t step = (int64_t)a.total_rows * heads;
+  f32x4_t v = none;
+  float top = kNegInf, sum = 0.0f;
+  if constexpr (SIDE == 1) {
+    for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * (row + s * step)]);
+    const float base = top == kNegInf ? 0.0f : top;
+    for (int s = 0; s < used; ++s) {
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (row + s * step)] - base);
+      sum += a.part_ml[2 * (row + s * step) + 1] * f;
+      v += *(const f32x4_t*)(a.part_o + (row + s * step) * D + d) * f;
+    }
+  } else {
+    f32x4_t p0 = none, p1 = none;
+    if (side < used) p0 = *(const f32x4_t*)(a.part_o + (row + side * step) * D + d);
+    if (side + SIDE < used) p1 = *(const f32x4_t*)(a.part_o + (row + (side + SIDE) * step) * D + d);
+    for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_ml[2 * (row + s * step)]);  // every wave by itself
+    top = wave_max(top);
+    const float base = top == kNegInf ? 0.0f : top;
+    for (int s = lane; s < used; s += 64) {
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (row + s * step)] - base);
+      sum += a.part_ml[2 * (row + s * step) + 1] * f;
+      if (tid < 64) s_f[s] = f;
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (side < used) v = p0 * s_f[side];
+    if (side + SIDE < used) v += p1 * s_f[side + SIDE];
+    for (int s = side + 2 * SIDE; s < used; s += SIDE)
+      v += *(const f32x4_t*)(a.part_o + (row + s * step) * D + d) * s_f[s];
+    s_v[side][tid % LPR] = v;
+    __syncthreads();
+    if (tid >= LPR) return;
+    for (int k = 1; k < SIDE; ++k) v += s_v[k][tid];
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
@@ -749,12 +824,13 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArg
 using namespace fdms;
 
 template <int D, bool FP8>
-static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, int tile_splits, hipStream_t st) {
+static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, int few_share, int tile_splits,
+                             hipStream_t st) {
   const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads, max_rows = (int64_t)max_seqlen * a.group;
   if (few_splits) {
     const dim3 grid((unsigned)(pairs * few_splits));
-    if (a.few_rows * a.group <= 16) block_attn_kernel<D, FP8, 1><<<grid, 256, 0, st>>>(a, few_splits);
-    else block_attn_kernel<D, FP8, 2><<<grid, 256, 0, st>>>(a, few_splits);
+    if (a.few_rows * a.group <= 16) block_attn_kernel<D, FP8, 1><<<grid, 256, 0, st>>>(a, few_splits, few_share);
+    else block_attn_kernel<D, FP8, 2><<<grid, 256, 0, st>>>(a, few_splits, few_share);
     FDMS_LAUNCH_CHECK();
   }
   if (tile_splits) {
@@ -764,8 +840,10 @@ static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, in
   }
   const int splits = few_splits > tile_splits ? few_splits : tile_splits;
   if (splits > 1) {
-    const int64_t rows = (int64_t)a.total_rows * a.num_kv_heads * a.group, per = 256 / (D / 4);
-    block_attn_join_kernel<D><<<dim3((unsigned)((rows - 1) / per + 1)), 256, 0, st>>>(a, splits);
+    const unsigned rows = (unsigned)a.total_rows * a.num_kv_heads * a.group;
+    constexpr int kSide = 1024 / D, kPer = 256 / (D / 4);
+    if (rows <= 2048) block_attn_join_kernel<D, kSide><<<dim3(rows), 256, 0, st>>>(a, splits);
+    else block_attn_join_kernel<D, 1><<<dim3((rows - 1) / kPer + 1), 256, 0, st>>>(a, splits);
     FDMS_LAUNCH_CHECK();
   }
   return 0;
@@ -778,7 +856,7 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
                                      const int32_t* context_lens, const int32_t* cu_seqlens, void* out, int64_t os_t,
                                      int64_t os_h, float* workspace, int num_seqs, int num_kv_heads, int group_size,
                                      int head_dim, int num_blocks, int block_size, int max_seqlen, int few_rows,
-                                     int few_splits, int tile_splits, float scale, void* stream) {
+                                     int few_splits, int few_share, int tile_splits, float scale, void* stream) {
   if ((q_dtype != kF16 && q_dtype != kBF16) || total_rows < 0 || num_seqs < 1 || num_kv_heads < 1 || group_size < 1 ||
       (head_dim != 64 && head_dim != 128) || max_seqlen < 1 || width < 0 || num_blocks < 1 || block_size < 16 ||
       block_size > 256 || (block_size & (block_size - 1)) ||
@@ -787,7 +865,7 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   // every sequence length has its kernel: up to few_rows query rows the one, past them the other
   const int splits = few_splits > tile_splits ? few_splits : tile_splits;
   if (few_rows < 0 || (int64_t)few_rows * group_size > 32 || few_splits < 0 || tile_splits < 0 || splits < 1 ||
-      splits > 1024 || (few_rows > 0 && few_splits == 0) || (few_rows < max_seqlen && tile_splits == 0) ||
+      splits > kMaxSplits || few_share < 1 || (few_rows > 0 && few_splits == 0) || (few_rows < max_seqlen && tile_splits == 0) ||
       (splits > 1 && workspace == nullptr))
     return (int)hipErrorInvalidValue;
   if (!fdms_aligned16(q, k_cache, v_cache, workspace) || (uintptr_t)out % 8 || qs_t % 8 || qs_h % 8 || os_t % 4 ||
@@ -796,7 +874,7 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads, max_rows = (int64_t)max_seqlen * group_size;
   const int64_t rows = (int64_t)total_rows * num_kv_heads * group_size;
   if (pairs * splits > 0x7FFFFFFF || (max_rows - 1) / kTileRows + 1 > 65535 || max_rows > 0x7FFFFFFF ||
-      (int64_t)total_rows * group_size > 0x7FFFFFFF || rows > 0x7FFFFFFFll * 4)
+      rows > 0x7FFFFFFF)
     return (int)hipErrorInvalidValue;
   if (total_rows == 0) return 0;
   BlockAttnArgs a;
@@ -814,7 +892,7 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   a.num_kv_heads = num_kv_heads, a.group = group_size, a.total_rows = total_rows;
   a.few_rows = few_rows, a.q_f16 = q_dtype == kF16, a.scale = scale;
   hipStream_t st = (hipStream_t)stream;
-#define FDMS_ATTN(D, F) return launch_block_attn<D, F>(a, max_seqlen, few_splits, tile_splits, st)
+#define FDMS_ATTN(D, F) return launch_block_attn<D, F>(a, max_seqlen, few_splits, few_share, tile_splits, st)
   if (head_dim == 64) {
     if (is_fp8) FDMS_ATTN(64, true);
     FDMS_ATTN(64, false);

@@ -237,29 +237,34 @@ def gather_block_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: 
 
 
 def block_attention_plan(seqs: int, heads: int, group: int, rows: int, max_seqlen: int,
-                         max_context: int) -> tuple[int, int, int]:
-    """(few_rows, few_splits, tile_splits) of a block_attention launch over
-    ``rows`` query rows: sequences of up to few_rows rows go to the kernel for
-    few rows, longer ones to the one for many; 0 splits leave a launch out.
+                         max_context: int) -> tuple[int, int, int, int]:
+    """(few_rows, few_splits, few_share, tile_splits) of a block_attention
+    launch over ``rows`` query rows: sequences of up to few_rows rows go to the
+    kernel for few rows, longer ones to the one for many; 0 splits leave a
+    launch out.
 
     A batch whose longest run has at most 32 rows x heads takes the first
     kernel alone, one sequence of more the second alone; several sequences may
     be of both kinds, and the first then takes those of at most 16.  Splits:
-    the first kernel to four workgroups per CU, each of at least 256 keys of
-    the longest context; the second those, each of at least 512 keys, that take
-    the least rounds x keys of the 512 workgroups (two per CU) the chip holds,
-    over the tiles that ``rows`` can make."""
+    the first kernel cuts every context into pieces of few_share 64-key groups,
+    as many as give three workgroups per CU if all were the longest, between 4
+    and 32; the second takes those, each of at least 512 keys, that take the
+    least rounds x keys of the 512 workgroups (two per CU) the chip holds, over
+    the tiles that ``rows`` can make."""
     pairs = seqs * heads
     if max_seqlen * group <= 32:
         few_rows = max_seqlen
     else:
         few_rows = 16 // group if seqs > 1 else 0
-    few = max(1, min(-(-1024 // pairs), -(-max_context // 256), 256)) if few_rows else 0
+    groups = -(-max_context // 64)
+    share = min(32, max(4, -(-groups * pairs // 768)))
+    share = max(share, -(-groups // 256))
+    few = max(1, -(-groups // share)) if few_rows else 0
     if few_rows >= max_seqlen:
-        return few_rows, few, 0
+        return few_rows, few, share, 0
     tiles = heads * (rows * group // 128 + seqs)
     most = max(1, min(-(-max_context // 512), 16)) if tiles < 1024 else 1
-    return few_rows, few, min(range(1, most + 1), key=lambda n: (-(-tiles * n // 512) + 0.1) / n + 0.01 * n)
+    return few_rows, few, share, min(range(1, most + 1), key=lambda n: (-(-tiles * n // 512) + 0.1) / n + 0.01 * n)
 
 
 def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -313,7 +318,7 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if t == 0:
         return out
     q = _aligned_rows(q)
-    few_rows, few_splits, tile_splits = block_attention_plan(n, h, hq // h, t, max_seqlen, max_context)
+    few_rows, few_splits, few_share, tile_splits = block_attention_plan(n, h, hq // h, t, max_seqlen, max_context)
     splits = max(few_splits, tile_splits)
     # the splits' partials, the call's own: nothing is shared between streams or captured graphs
     ws = torch.empty(t * hq * (splits * (d + 2) + 1), device=dev, dtype=torch.float32) if splits > 1 else None
@@ -322,5 +327,6 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(),
             k_scale.stride(0), block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(),
             nat.ptr(cu_seqlens), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), n, h, hq // h, d, nb, bs,
-            max_seqlen, few_rows, few_splits, tile_splits, d ** -0.5 if scale is None else float(scale))
+            max_seqlen, few_rows, few_splits, few_share, tile_splits,
+            d ** -0.5 if scale is None else float(scale))
     return out

@@ -674,8 +674,8 @@ int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_f
  * sees no key gets zeros; rows outside cu_seqlens are not written.  q rows
  * 16-byte, out rows 8-byte aligned.  Sequences of up to few_rows
  * query rows (few_rows * group_size <= 32) run on the kernel for few rows with
- * their keys in up to few_splits parts, longer ones on the one for many with
- * up to tile_splits; a count of 0 leaves a launch out and is refused where a
+ * their keys in parts of about few_share groups of 64, at most few_splits, longer ones on the one for many with
+ * up to tile_splits (both at most 256); a count of 0 leaves a launch out and is refused where a
  * sequence may need it.  With S the larger count above 1 the workspace holds
  * S * total_rows * heads * group_size * (D + 2) + total_rows * heads *
  * group_size floats (16-byte aligned) that no other call may use meanwhile. */
@@ -685,8 +685,8 @@ int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, int64_t qs_h,
                          const int32_t* block_tables, int64_t bt_b, int width, const int32_t* context_lens,
                          const int32_t* cu_seqlens, void* out, int64_t os_t, int64_t os_h, float* workspace,
                          int num_seqs, int num_kv_heads, int group_size, int head_dim, int num_blocks,
-                         int block_size, int max_seqlen, int few_rows, int few_splits, int tile_splits,
-                         float scale, void* stream);
+                         int block_size, int max_seqlen, int few_rows, int few_splits, int few_share,
+                         int tile_splits, float scale, void* stream);
 
 #ifdef __cplusplus
 }
