@@ -122,6 +122,12 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """Handle of GPU ``index``'s current stream, as stream() gives it for the
+    current device, without building a Stream object (0.1 against 2.8 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_cuda(*tensors: torch.Tensor, what: str = "fastdms_amd op") -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -147,37 +147,33 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
 //
 // Bound by HBM: 4 bytes read per value pair and 2 written; a prompt's blocks
 // are independent, so the grid covers them all at once.
-constexpr int kKPass = 4;  // at most: passes of 64 lanes over a 16-row K tile of 8-channel pieces
-
-template <typename T>
-__device__ __forceinline__ void load_row8(const T* p, float* x) {
-  if constexpr (sizeof(T) == 2) {
-    const u32x4_t r = *(const u32x4_t*)p;
-    const T* e = (const T*)&r;
+// N row elements as loaded (two to a register where they are halves), and as fp32.
+template <typename T, int N>
+struct Raw {
+  static constexpr int W = N * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ld<T>(e + i);
-  } else {
+      for (int i = 0; i < W; i += 4) {
+        const u32x4_t r = *(const u32x4_t*)(p + i * 4 / sizeof(T));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4_t r = *(const f32x4_t*)(p + 4 * h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = r[i];
+        for (int j = 0; j < 4; ++j) w[i + j] = r[j];
+      }
+    } else if constexpr (W == 2) {
+      const u32x2_t r = *(const u32x2_t*)p;
+      w[0] = r[0];
+      w[1] = r[1];
+    } else {
+      w[0] = *(const uint32_t*)p;
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void load_pair(const T* p, float* x0, float* x1) {
-  if constexpr (sizeof(T) == 2) {
-    const uint32_t r = *(const uint32_t*)p;
-    const T* e = (const T*)&r;
-    *x0 = ld<T>(e);
-    *x1 = ld<T>(e + 1);
-  } else {
-    const f32x2_t r = *(const f32x2_t*)p;
-    *x0 = r[0];
-    *x1 = r[1];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const uint16_t e = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    return ld<T>((const T*)&e);
   }
-}
+};
 
 // Max over the workgroup (WAVES waves); every thread calls it.
 template <int WAVES>
@@ -194,6 +190,30 @@ __device__ __forceinline__ float team_max(float v, float* s_red) {
   return v;
 }
 
+// Codes of four values x, times inv = 1 / scale.  A wave all of whose values are
+// finite needs neither clamp nor NaN test: |x| / scale is at most the largest
+// code.  int8 then takes one fma per value, whose sum with 1.5 * 2^23 holds
+// the rounded integer in its low byte (x / scale is exact, so it rounds once).
+template <bool FP8>
+__device__ __forceinline__ uint32_t encode4_finite(float a, float b, float c, float d, float inv) {
+  if constexpr (FP8) {
+    const uint32_t r = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, (int)r, true);
+  }
+  const float k = 12582912.0f;
+  const uint32_t x = __float_as_uint(__builtin_fmaf(a, inv, k)), y = __float_as_uint(__builtin_fmaf(b, inv, k));
+  const uint32_t z = __float_as_uint(__builtin_fmaf(c, inv, k)), w = __float_as_uint(__builtin_fmaf(d, inv, k));
+  // perm selects from (second operand bytes 0-3, first operand bytes 4-7)
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0C0C0400u), __builtin_amdgcn_perm(y, x, 0x0C0C0400u),
+                               0x05040100u);
+}
+// Four codes of a block whose scale has grown (ratio: old / new, below 1).
+template <bool FP8>
+__device__ __forceinline__ uint32_t encode4_again(uint32_t c, float ratio) {
+  return encode4<FP8>(code_value<FP8>(c, 0) * ratio, code_value<FP8>(c, 1) * ratio, code_value<FP8>(c, 2) * ratio,
+                      code_value<FP8>(c, 3) * ratio);
+}
+
 // The scale of a block after a run's rows (amax) joined `off` earlier ones.
 template <bool FP8>
 __device__ __forceinline__ float joined_scale(float amax, int off, float old) {
@@ -205,23 +225,44 @@ template <typename T, int D, bool FP8, int WAVES>
 __device__ __forceinline__ void store_run_k(const T* __restrict__ x, int64_t xs_t, uint8_t* block, float* scale,
                                             int off, int n, float* s_red) {
   constexpr int LPR = D / 8, RPP = kWave / LPR, PASS = kTile / RPP;
-  static_assert(PASS <= kKPass, "tile passes");
-  const int lane = lane_id(), row0 = (threadIdx.x >> 6) * kTile + lane / LPR, d0 = (lane % LPR) * 8;
-  float v[PASS][8], amax = 0.0f;
+  const int lane = lane_id(), tile0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kTile;
+  const int row0 = tile0 + lane / LPR, d0 = (lane % LPR) * 8;
+  const float old = *scale;
+  Raw<T, 8> v[PASS] = {};
+  float amax = 0.0f, odd = 0.0f;  // odd: NaN once a value is infinite or NaN
+  if (tile0 < off + n && tile0 + kTile > off) {  // some of the wave's rows are new
+    if (tile0 >= off && tile0 + kTile <= off + n) {  // all of them: one address per lane, the passes at scalar steps
+      const T* p = x + (int64_t)(row0 - off) * xs_t + d0;
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int r = row0 + i * RPP;
-    if (r >= off && r < off + n) {
-      load_row8<T>(x + (int64_t)(r - off) * xs_t + d0, v[i]);
+      for (int i = 0; i < PASS; ++i) v[i].load(p + i * RPP * xs_t);
+    } else {  // rows past the run are its first or last again
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) v[i].load(x + (int64_t)min(max(row0 + i * RPP - off, 0), n - 1) * xs_t + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < PASS; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[i][j] = nan_to_zero(v[i][j]);
         amax = fmaxf(amax, fabsf(v[i][j]));
+        odd = __builtin_fmaf(v[i][j], 0.0f, odd);
       }
-    }
   }
-  const float old = *scale, s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old);
-  const float inv = 1.0f / s;
+  const float s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old), inv = 1.0f / s;
+  u32x2_t c[PASS];
+  if (!__any(odd != odd)) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        c[i][j] = encode4_finite<FP8>(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3], inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        c[i][j] = encode4<FP8>(nan_to_zero(v[i][4 * j]) * inv, nan_to_zero(v[i][4 * j + 1]) * inv,
+                               nan_to_zero(v[i][4 * j + 2]) * inv, nan_to_zero(v[i][4 * j + 3]) * inv);
+  }
   const bool grown = off > 0 && s > old;
   const float ratio = old * inv;
 #pragma unroll
@@ -229,19 +270,12 @@ __device__ __forceinline__ void store_run_k(const T* __restrict__ x, int64_t xs_
     const int r = row0 + i * RPP;
     u32x2_t* dst = (u32x2_t*)(block + r * D + d0);
     if (r >= off && r < off + n) {
-      u32x2_t c;
-      c[0] = encode4<FP8>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-      c[1] = encode4<FP8>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-      *dst = c;
+      *dst = c[i];
     } else if (grown && r < off) {
-      u32x2_t c = *dst;
+      u32x2_t was = *dst;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t w = c[j];
-        c[j] = encode4<FP8>(code_value<FP8>(w, 0) * ratio, code_value<FP8>(w, 1) * ratio,
-                            code_value<FP8>(w, 2) * ratio, code_value<FP8>(w, 3) * ratio);
-      }
-      *dst = c;
+      for (int j = 0; j < 2; ++j) was[j] = encode4_again<FP8>(was[j], ratio);
+      *dst = was;
     }
   }
   if (threadIdx.x == 0) *scale = s;
@@ -253,54 +287,71 @@ template <typename T, int D, bool FP8, int WAVES>
 __device__ __forceinline__ void store_run_v(const T* __restrict__ x, int64_t xs_t, uint8_t* block, float* scale,
                                             int off, int n, float* s_red) {
   constexpr int LPR = D / 2, TOK = kTile * LPR / kWave, WORDS = TOK / 4;
-  const int lane = lane_id(), tile = threadIdx.x >> 6, d0 = (lane % LPR) * 2, t0 = (lane / LPR) * TOK;
-  const int row0 = tile * kTile + t0;
-  float v[2][TOK], amax = 0.0f;
+  typedef uint32_t words_t __attribute__((ext_vector_type(WORDS)));
+  const int lane = lane_id(), tile0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kTile;
+  const int d0 = (lane % LPR) * 2, t0 = (lane / LPR) * TOK, row0 = tile0 + t0;
+  const float old = *scale;
+  Raw<T, 2> v[TOK] = {};
+  float amax = 0.0f, odd = 0.0f;
+  if (tile0 < off + n && tile0 + kTile > off) {
+    if (tile0 >= off && tile0 + kTile <= off + n) {
+      const T* p = x + (int64_t)(row0 - off) * xs_t + d0;
 #pragma unroll
-  for (int j = 0; j < TOK; ++j) {
-    const int r = row0 + j;
-    v[0][j] = v[1][j] = 0.0f;
-    if (r >= off && r < off + n) {
-      load_pair<T>(x + (int64_t)(r - off) * xs_t + d0, &v[0][j], &v[1][j]);
-      v[0][j] = nan_to_zero(v[0][j]);
-      v[1][j] = nan_to_zero(v[1][j]);
-      amax = fmaxf(amax, fmaxf(fabsf(v[0][j]), fabsf(v[1][j])));
+      for (int j = 0; j < TOK; ++j) v[j].load(p + j * xs_t);
+    } else {
+#pragma unroll
+      for (int j = 0; j < TOK; ++j) v[j].load(x + (int64_t)min(max(row0 + j - off, 0), n - 1) * xs_t + d0);
+    }
+#pragma unroll
+    for (int j = 0; j < TOK; ++j) {
+      amax = fmaxf(amax, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
+      odd = __builtin_fmaf(v[j][0], 0.0f, odd);
+      odd = __builtin_fmaf(v[j][1], 0.0f, odd);
     }
   }
-  const float old = *scale, s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old);
-  const float inv = 1.0f / s;
+  const float s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old), inv = 1.0f / s;
   const bool grown = off > 0 && s > old;
-  const float ratio = old * inv;
-  const bool any_new = row0 < off + n && row0 + TOK > off;
-  if (any_new || (grown && row0 < off)) {
-    const bool whole = row0 >= off && row0 + TOK <= off + n;
+  if (threadIdx.x == 0) *scale = s;
+  if (!(row0 < off + n && row0 + TOK > off) && !(grown && row0 < off)) return;  // nothing of the lane's changes
+  words_t code[2];
+  if (!__any(odd != odd)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w)
+        code[c][w] = encode4_finite<FP8>(v[4 * w][c], v[4 * w + 1][c], v[4 * w + 2][c], v[4 * w + 3][c], inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w)
+        code[c][w] = encode4<FP8>(nan_to_zero(v[4 * w][c]) * inv, nan_to_zero(v[4 * w + 1][c]) * inv,
+                                  nan_to_zero(v[4 * w + 2][c]) * inv, nan_to_zero(v[4 * w + 3][c]) * inv);
+  }
+  words_t* dst = (words_t*)(block + tile0 * D + d0 * kTile + t0);
+  constexpr int STEP = kTile / (4 * WORDS);  // words_t's from a channel's tokens to the next one's
+  if (!(row0 >= off && row0 + TOK <= off + n)) {
+    // bytes of the rows before (encoded again if the scale grew) and of those behind
+    const float ratio = old * inv;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      uint32_t* dst = (uint32_t*)(block + (int64_t)tile * (D * kTile) + (d0 + c) * kTile + t0);
+      const words_t was = dst[c * STEP];
 #pragma unroll
       for (int w = 0; w < WORDS; ++w) {
-        uint32_t code = encode4<FP8>(v[c][4 * w] * inv, v[c][4 * w + 1] * inv, v[c][4 * w + 2] * inv,
-                                     v[c][4 * w + 3] * inv);
-        if (!whole) {  // bytes of the rows before (encoded again if the scale grew) and of those behind
-          const uint32_t was = dst[w];
-          uint32_t again = was;
-          if (grown)
-            again = encode4<FP8>(code_value<FP8>(was, 0) * ratio, code_value<FP8>(was, 1) * ratio,
-                                 code_value<FP8>(was, 2) * ratio, code_value<FP8>(was, 3) * ratio);
-          uint32_t mixed = 0;
+        const uint32_t again = grown ? encode4_again<FP8>(was[w], ratio) : was[w];
+        uint32_t mixed = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = row0 + 4 * w + j;
-            const uint32_t from = r < off ? again : (r < off + n ? code : was);
-            mixed |= from & (0xFFu << (8 * j));
-          }
-          code = mixed;
+        for (int j = 0; j < 4; ++j) {
+          const int r = row0 + 4 * w + j;
+          const uint32_t from = r < off ? again : (r < off + n ? code[c][w] : was[w]);
+          mixed |= from & (0xFFu << (8 * j));
         }
-        dst[w] = code;
+        code[c][w] = mixed;
       }
     }
   }
-  if (threadIdx.x == 0) *scale = s;
+  dst[0] = code[0];
+  dst[STEP] = code[1];
 }
 
 template <typename T, int D, bool FP8, int WAVES>
@@ -308,12 +359,14 @@ __global__ __launch_bounds__(64 * WAVES) void store_block_kernel(
     const T* __restrict__ k, int64_t ks_t, int64_t ks_h, const T* __restrict__ v, int64_t vs_t, int64_t vs_h,
     uint8_t* kc, int64_t kc_b, int64_t kc_h, uint8_t* vc, int64_t vc_b, int64_t vc_h, float* k_scale,
     float* v_scale, int64_t sc_b, const int32_t* __restrict__ slots,
-    int num_tokens, int num_blocks, int per_group) {
+    int num_tokens, int num_blocks, int num_heads, int per_group) {
   constexpr int BS = kTile * WAVES;
   __shared__ float s_red[WAVES];
-  const int h = blockIdx.y, lane = lane_id();
-  const bool is_v = blockIdx.z != 0;
-  int64_t t = (int64_t)blockIdx.x * per_group;
+  // heads, and K and V, run fastest: workgroups that run together read whole rows of the projection
+  const unsigned heads2 = 2 * num_heads, part = blockIdx.x % heads2;
+  const int h = part % num_heads, lane = lane_id();
+  const bool is_v = part >= (unsigned)num_heads;
+  int64_t t = (int64_t)(blockIdx.x / heads2) * per_group;
   const int64_t end = min(t + per_group, (int64_t)num_tokens);
   while (t < end) {
     const int slot = slots[t];
@@ -324,13 +377,18 @@ __global__ __launch_bounds__(64 * WAVES) void store_block_kernel(
     }
     const bool first = off == 0 || t == 0 || slots[t - 1] != slot - 1;
     int n = 0;  // rows of the run: the leading lanes whose slots follow on
-    for (int i0 = 0; i0 < BS; i0 += kWave) {
-      const int i = i0 + lane;
-      const bool on = off + i < BS && t + i < num_tokens && slots[t + i] == slot + i;
-      const uint64_t m = ~__ballot(on);
+    constexpr int LOOKS = (BS + kWave - 1) / kWave;
+    int seen[LOOKS];
+#pragma unroll
+    for (int k = 0; k < LOOKS; ++k) seen[k] = slots[min(t + k * kWave + lane, (int64_t)num_tokens - 1)];
+    bool whole = true;
+#pragma unroll
+    for (int k = 0; k < LOOKS; ++k) {
+      const int i = k * kWave + lane;
+      const uint64_t m = ~__ballot(off + i < BS && t + i < num_tokens && seen[k] == slot + i);
       const int run = m ? __builtin_ctzll(m) : kWave;
-      n += run;
-      if (run < kWave) break;
+      n += whole ? run : 0;
+      whole = whole && run == kWave;
     }
     if (first) {
       if (is_v)
@@ -346,60 +404,119 @@ __global__ __launch_bounds__(64 * WAVES) void store_block_kernel(
 
 // ------------------------------------------------------------------ read-back
 // Dense rows of the tokens at slots[t]; a slot outside the cache gives zeros.
-// A wave takes 16 tokens of one kv head, K or V.  V comes from transposed
-// tiles: a lane keeps the 16 tokens of its two channels in registers while the
-// tokens stay in one tile, so a run of slots reads each tile once.
+// A wave takes 16 tokens of one kv head, K or V, every load on its way before
+// the first is looked at.  K: 16 bytes of a row per lane.  V comes from
+// transposed tiles: a lane holds the 16 tokens of two channels of the tiles that
+// its first and last token lie in -- a run of slots has no others -- and looks up
+// single bytes of any further ones.
+// Two values as TO's, to nearest even by the hardware (v_cvt_pk_bf16_f32, v_cvt_pk_f16_f32).
+template <typename TO> struct Pair;
+template <> struct Pair<float> {
+  typedef u32x2_t bits;
+  static __device__ __forceinline__ bits of(float a, float b) { return bits{__float_as_uint(a), __float_as_uint(b)}; }
+};
+template <> struct Pair<f16_t> {
+  typedef uint32_t bits;
+  static __device__ __forceinline__ bits of(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
+  }
+};
+template <> struct Pair<bf16_t> {
+  typedef uint32_t bits;
+  typedef __bf16 two __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ bits of(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), two));
+  }
+};
+
+// The 8-bit codes' values exactly, by the hardware's conversion (e4m3fn) or a byte's (int8).
+template <bool FP8, int I>
+__device__ __forceinline__ float code_value_at(uint32_t c) {
+  if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8((int)c, I);
+  return (float)((int)(c << (24 - 8 * I)) >> 24);
+}
+
 template <typename TO, int D, bool FP8>
 __global__ __launch_bounds__(256) void gather_block_kernel(
     const uint8_t* __restrict__ kc, int64_t kc_b, int64_t kc_h, const uint8_t* __restrict__ vc, int64_t vc_b,
     int64_t vc_h, const float* __restrict__ k_scale, const float* __restrict__ v_scale, int64_t sc_b,
     const int32_t* __restrict__ slots, int num_tokens, int num_blocks, int shift, TO* __restrict__ out_k,
-    int64_t ok_t, int64_t ok_h, TO* __restrict__ out_v, int64_t ov_t, int64_t ov_h) {
-  constexpr int LPR = D / 2, TOK = kTile * LPR / kWave;  // lanes per row, tokens per lane
-  const int h = blockIdx.y, lane = lane_id();
-  const bool is_v = blockIdx.z != 0;
-  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kTile + (lane / LPR) * TOK;
-  const int d0 = (lane % LPR) * 2;
-  const int mask = (1 << shift) - 1;
-  TO* out = is_v ? out_v : out_k;
-  const int64_t os_t = is_v ? ov_t : ok_t, os_h = is_v ? ov_h : ok_h;
-  int tile = -1;
-  u32x4_t c0 = {0, 0, 0, 0}, c1 = {0, 0, 0, 0};
-  float s = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < TOK; ++i) {
-    const int64_t t = t0 + i;
-    if (t >= num_tokens) break;
-    const int slot = slots[t];
-    const int blk = slot >> shift, off = slot & mask;
-    float x0 = 0.0f, x1 = 0.0f;
-    if (slot >= 0 && blk < num_blocks) {
-      if (is_v) {
-        if (slot >> 4 != tile) {
-          tile = slot >> 4;
-          const u32x4_t* p = (const u32x4_t*)(vc + blk * vc_b + h * vc_h + (off >> 4) * (D * kTile) + d0 * kTile);
-          c0 = p[0];
-          c1 = p[1];
-          s = v_scale[blk * sc_b + h];
-        }
-        const int w = (off >> 2) & 3;
-        const uint32_t a = w == 0 ? c0[0] : w == 1 ? c0[1] : w == 2 ? c0[2] : c0[3];
-        const uint32_t b = w == 0 ? c1[0] : w == 1 ? c1[1] : w == 2 ? c1[2] : c1[3];
-        x0 = code_value<FP8>(a, off & 3) * s;
-        x1 = code_value<FP8>(b, off & 3) * s;
-      } else {
-        const uint32_t c = *(const uint16_t*)(kc + blk * kc_b + h * kc_h + off * D + d0);
-        s = k_scale[blk * sc_b + h];
-        x0 = code_value<FP8>(c, 0) * s;
-        x1 = code_value<FP8>(c, 1) * s;
-      }
+    int64_t ok_t, int64_t ok_h, TO* __restrict__ out_v, int64_t ov_t, int64_t ov_h, int num_heads) {
+  const unsigned chunks = gridDim.x / (2u * num_heads), part = blockIdx.x / chunks;
+  const int h = part % num_heads, lane = lane_id(), mask = (1 << shift) - 1;
+  const bool is_v = part >= (unsigned)num_heads;
+  const int64_t first = ((int64_t)(blockIdx.x % chunks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kTile;
+  if (first >= num_tokens) return;
+  const int left = (int)min((int64_t)num_tokens - first, (int64_t)kTile);
+  // lane i holds token i % 16: its slot (-1 outside the cache) and scale
+  int slot = slots[first + min(lane & 15, left - 1)];
+  if (slot < 0 || slot >> shift >= num_blocks) slot = -1;
+  const float* scales = is_v ? v_scale : k_scale;
+  const float sc = slot < 0 ? 0.0f : scales[(int64_t)(slot >> shift) * sc_b + h];
+  if (!is_v) {
+    constexpr int LPR = D / 16, RPP = kWave / LPR, PASS = kTile / RPP;
+    u32x4_t c[PASS];
+    int sl[PASS];
+    float s[PASS];
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int row = i * RPP + lane / LPR;
+      sl[i] = __shfl(slot, row, kWave);
+      s[i] = __shfl(sc, row, kWave);
+      const int at = max(sl[i], 0);
+      c[i] = *(const u32x4_t*)(kc + (int64_t)(at >> shift) * kc_b + h * kc_h + (at & mask) * D + (lane % LPR) * 16);
     }
-    TO pair[2];
-    st<TO>(&pair[0], x0);
-    st<TO>(&pair[1], x1);
-    TO* dst = out + t * os_t + h * os_h + d0;
-    if constexpr (sizeof(TO) == 2) *(uint32_t*)dst = __builtin_bit_cast(uint32_t, pair);
-    else *(u32x2_t*)dst = __builtin_bit_cast(u32x2_t, pair);
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int row = i * RPP + lane / LPR;
+      if (row >= left) continue;
+      TO* dst = out_k + (first + row) * ok_t + h * ok_h + (lane % LPR) * 16;
+      typename Pair<TO>::bits e[8];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t x = sl[i] < 0 ? 0u : c[i][w];
+        e[2 * w] = Pair<TO>::of(code_value_at<FP8, 0>(x) * s[i], code_value_at<FP8, 1>(x) * s[i]);
+        e[2 * w + 1] = Pair<TO>::of(code_value_at<FP8, 2>(x) * s[i], code_value_at<FP8, 3>(x) * s[i]);
+      }
+#pragma unroll
+      for (int w = 0; w < (int)sizeof(TO); ++w) ((u32x4_t*)dst)[w] = ((const u32x4_t*)e)[w];
+    }
+    return;
+  }
+  constexpr int LPR = D / 2, TOK = kTile * LPR / kWave;  // lanes per row, tokens per lane
+  const int t0 = (lane / LPR) * TOK, d0 = (lane % LPR) * 2;
+  auto tile_at = [&](int s) {  // the lane's channels of the tile that holds a slot
+    const int at = max(s, 0);
+    return (const u32x4_t*)(vc + (int64_t)(at >> shift) * vc_b + h * vc_h + ((at & mask) >> 4) * (D * kTile) +
+                            d0 * kTile);
+  };
+  int sl[TOK];
+  float s[TOK];
+#pragma unroll
+  for (int j = 0; j < TOK; ++j) {
+    sl[j] = __shfl(slot, t0 + j, kWave);
+    s[j] = __shfl(sc, t0 + j, kWave);
+  }
+  const int a_tile = sl[0] >> 4, b_tile = sl[TOK - 1] >> 4;
+  const u32x4_t a0 = tile_at(sl[0])[0], a1 = tile_at(sl[0])[1];
+  const u32x4_t b0 = tile_at(sl[TOK - 1])[0], b1 = tile_at(sl[TOK - 1])[1];
+#pragma unroll
+  for (int j = 0; j < TOK; ++j) {
+    if (t0 + j >= left) break;
+    const int tile = sl[j] >> 4, w = (sl[j] >> 2) & 3, sh = 8 * (sl[j] & 3);
+    uint32_t x, y;
+    if (tile == a_tile || tile == b_tile) {
+      const u32x4_t c0 = tile == a_tile ? a0 : b0, c1 = tile == a_tile ? a1 : b1;
+      x = (w & 2 ? (w & 1 ? c0[3] : c0[2]) : (w & 1 ? c0[1] : c0[0])) >> sh;
+      y = (w & 2 ? (w & 1 ? c1[3] : c1[2]) : (w & 1 ? c1[1] : c1[0])) >> sh;
+    } else {
+      const uint8_t* p = (const uint8_t*)tile_at(sl[j]) + (sl[j] & 15);
+      x = p[0];
+      y = p[kTile];
+    }
+    if (sl[j] < 0) x = y = 0;
+    *(typename Pair<TO>::bits*)(out_v + (first + t0 + j) * ov_t + h * ov_h + d0) =
+        Pair<TO>::of(code_value_at<FP8, 0>(x) * s[j], code_value_at<FP8, 0>(y) * s[j]);
   }
 }
 
@@ -438,12 +555,12 @@ template <typename T, int D, bool FP8>
 static int launch_store(int block_size, dim3 grid, hipStream_t st, const void* k, int64_t ks_t, int64_t ks_h,
                         const void* v, int64_t vs_t, int64_t vs_h, void* kc, int64_t kc_b, int64_t kc_h, void* vc,
                         int64_t vc_b, int64_t vc_h, float* k_scale, float* v_scale, int64_t sc_b,
-                        const int32_t* slots, int num_tokens, int num_blocks, int per_group) {
+                        const int32_t* slots, int num_tokens, int num_blocks, int num_heads, int per_group) {
 #define FDMS_STORE(W)                                                                                             \
   store_block_kernel<T, D, FP8, W><<<grid, 64 * W, 0, st>>>((const T*)k, ks_t, ks_h, (const T*)v, vs_t, vs_h,     \
                                                             (uint8_t*)kc, kc_b, kc_h, (uint8_t*)vc, vc_b, vc_h,   \
                                                             k_scale, v_scale, sc_b, slots, num_tokens, num_blocks, \
-                                                            per_group)
+                                                            num_heads, per_group)
   switch (block_size / kTile) {
     case 1: FDMS_STORE(1); break;
     case 2: FDMS_STORE(2); break;
@@ -462,7 +579,8 @@ FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int
                                          float* v_scale, int64_t sc_b, const int32_t* slot_mapping, int num_tokens,
                                          int num_blocks, int block_size, int num_kv_heads, int head_dim,
                                          void* stream) {
-  if (dtype < kF32 || dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 || num_kv_heads > 65535)
+  if (dtype < kF32 || dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 ||
+      ((int64_t)num_tokens / 16 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
     return (int)hipErrorInvalidValue;
   if (!block_cache_ok(k_cache, kc_b, kc_h, v_cache, vc_b, vc_h, num_blocks, block_size, head_dim))
     return (int)hipErrorInvalidValue;
@@ -474,10 +592,10 @@ FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int
   // workgroups then find one or two each.  A step of few tokens, whose rows
   // lie in a block each, gets a workgroup per token, so none stores several.
   const int per_group = num_tokens <= 512 ? 1 : block_size;
-  const dim3 grid((num_tokens - 1) / per_group + 1, num_kv_heads, 2);
+  const dim3 grid(((num_tokens - 1) / per_group + 1) * 2u * num_kv_heads);
 #define FDMS_ARGS                                                                                                 \
   block_size, grid, (hipStream_t)stream, key, ks_t, ks_h, value, vs_t, vs_h, k_cache, kc_b, kc_h, v_cache, vc_b,  \
-      vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, num_blocks, per_group
+      vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, num_blocks, num_kv_heads, per_group
   FDMS_DISPATCH_FLOAT(dtype, T, {
     if (head_dim == 64) return is_fp8 ? launch_store<T, 64, true>(FDMS_ARGS) : launch_store<T, 64, false>(FDMS_ARGS);
     return is_fp8 ? launch_store<T, 128, true>(FDMS_ARGS) : launch_store<T, 128, false>(FDMS_ARGS);
@@ -492,22 +610,21 @@ FDMS_EXPORT int fdms_gather_block_kvcache(const void* k_cache, const void* v_cac
                                           int num_tokens, int num_blocks, int block_size, int num_kv_heads,
                                           int head_dim, void* out_k, void* out_v, int out_dtype, int64_t ok_t,
                                           int64_t ok_h, int64_t ov_t, int64_t ov_h, void* stream) {
-  if (out_dtype < kF32 || out_dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 || num_kv_heads > 65535)
+  if (out_dtype < kF32 || out_dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 ||
+      ((int64_t)num_tokens / 16 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
     return (int)hipErrorInvalidValue;
   if (!block_cache_ok(k_cache, kc_b, kc_h, v_cache, vc_b, vc_h, num_blocks, block_size, head_dim))
     return (int)hipErrorInvalidValue;
-  const int64_t pair = out_dtype == kF32 ? 8 : 4;  // bytes a lane stores
-  if ((uintptr_t)out_k % pair || (uintptr_t)out_v % pair || (ok_t | ok_h | ov_t | ov_h) % 2)
-    return (int)hipErrorInvalidValue;
+  if (!fdms_aligned16(out_k, out_v) || (ok_t | ok_h | ov_t | ov_h) % 8) return (int)hipErrorInvalidValue;
   if (num_tokens == 0) return 0;
-  const dim3 grid((num_tokens - 1) / (4 * kTile) + 1, num_kv_heads, 2);
+  const dim3 grid(((num_tokens - 1) / (4 * kTile) + 1) * 2u * num_kv_heads);
   const int shift = __builtin_ctz(block_size);
   hipStream_t st = (hipStream_t)stream;
 #define FDMS_GATHER(TT, D, F)                                                                                     \
   gather_block_kernel<TT, D, F><<<grid, 256, 0, st>>>((const uint8_t*)k_cache, kc_b, kc_h, (const uint8_t*)v_cache, \
                                                      vc_b, vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, \
                                                      num_blocks, shift, (TT*)out_k, ok_t, ok_h, (TT*)out_v, ov_t,  \
-                                                     ov_h)
+                                                     ov_h, num_kv_heads)
   FDMS_DISPATCH_FLOAT(out_dtype, T, {
     if (head_dim == 64) {
       if (is_fp8) FDMS_GATHER(T, 64, true);

@@ -75,34 +75,40 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int
         raise ValueError(f"expected v_cache {(nb, h, bs // TILE, d, TILE)}, got {tuple(v_cache.shape)}")
     if nb < 1 or nb * bs > _INT_MAX:
         raise ValueError("a block KV cache needs at least one block and fewer than 2^31 slots")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if ks[3] != 1 or ks[2] != d or vs[4] != 1 or vs[3] != TILE or (bs > TILE and vs[2] != TILE * d):
+    kb, kh, kr, kd = k_cache.stride()
+    vb, vh, vt, vd, vi = v_cache.stride()
+    if kd != 1 or kr != d or vi != 1 or vd != TILE or (bs > TILE and vt != TILE * d):
         raise ValueError("a head's part of a block must be contiguous in k_cache and v_cache")
-    if (ks[0] | ks[1] | vs[0] | vs[1] | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+    if (kb | kh | vb | vh | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError("k_cache and v_cache blocks must be 16-byte aligned")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or s.shape != (nb, h) or (h > 1 and s.stride(1) != 1):
-            raise ValueError(f"expected fp32 scales [{nb}, {h}] with contiguous heads")
-    if nb > 1 and k_scale.stride(0) != v_scale.stride(0):
-        raise ValueError("k_scale and v_scale must have the same block stride")
+    if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or \
+            k_scale.shape != (nb, h) or v_scale.shape != (nb, h):
+        raise ValueError(f"expected fp32 scales [{nb}, {h}], got {k_scale.dtype} {tuple(k_scale.shape)} and "
+                         f"{v_scale.dtype} {tuple(v_scale.shape)}")
+    sb, sh = k_scale.stride()
+    tb, th = v_scale.stride()
+    if h > 1 and (sh != 1 or th != 1) or nb > 1 and sb != tb:
+        raise ValueError("k_scale and v_scale need contiguous heads and the same block stride")
     return nb, h, bs, d
 
 
-def _on_device(what: str, *tensors) -> torch.device:
-    dev = tensors[0].device
+def _device_index(what: str, *tensors) -> int:
+    """The index of the one GPU that holds all tensors."""
+    i = tensors[0].get_device()
     for t in tensors:
-        if t.device != dev or dev.type != "cuda":
-            raise RuntimeError(f"{what} requires its tensors on one GPU (HIP device); got {t.device} and {dev}")
-    return dev
+        if t.get_device() != i or i < 0:
+            raise RuntimeError(f"{what} requires its tensors on one GPU (HIP device); got {t.device} and "
+                               f"{tensors[0].device}")
+    return i
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
+def _launch(index: int, name: str, *args) -> None:
     """nat.call on the tensors' device, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        nat.call(name, *args, nat.stream())
+    if index == torch.cuda.current_device():
+        nat.call(name, *args, nat.raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            nat.call(name, *args, nat.stream())
+        with torch.cuda.device(index):
+            nat.call(name, *args, nat.raw_stream(index))
 
 
 def _int32(what: str, t: torch.Tensor, shape: tuple) -> None:
@@ -148,11 +154,11 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
     if not 0 <= num_tokens <= _INT_MAX:
         raise ValueError(f"num_tokens must be between 0 and {_INT_MAX}, got {num_tokens}")
-    dev = _on_device("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count)
+    dev = _device_index("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count)
     if out is None:
-        slots, cu, ctx, count, status = torch.empty(num_tokens + 2 * n + 3, device=dev, dtype=torch.int32).split(
+        slots, cu, ctx, count, status = cached_lens.new_empty(num_tokens + 2 * n + 3).split(
             (num_tokens, n + 1, n, 1, 1))
-        out = BlockTables(slots, torch.empty(num_tokens, device=dev, dtype=torch.int64), cu, ctx, count, status)
+        out = BlockTables(slots, cached_lens.new_empty(num_tokens, dtype=torch.int64), cu, ctx, count, status)
     else:
         for what, size in (("slot_mapping", num_tokens), ("cu_seqlens", n + 1), ("context_lens", n),
                            ("free_count", 1), ("status", 1)):
@@ -160,7 +166,7 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
         if out.positions.dtype != torch.int64 or out.positions.shape != (num_tokens,) or \
                 not out.positions.is_contiguous():
             raise ValueError(f"out.positions must be a contiguous int64 [{num_tokens}] tensor")
-        _on_device("prepare_block_tables", cached_lens, *out)
+        _device_index("prepare_block_tables", cached_lens, *out)
         if out.free_count.data_ptr() == free_count.data_ptr():
             raise ValueError("out.free_count must be another tensor than free_count")
     _launch(dev, "fdms_block_tables", cached_lens.data_ptr(), new_lens.data_ptr(), n, block_tables.data_ptr(),
@@ -172,10 +178,17 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     """x [rows, heads, D] with a contiguous head_dim and 16-byte aligned rows: itself, or a copy."""
-    size = x.element_size()
-    if x.stride(2) == 1 and not (x.stride(0) * size | x.stride(1) * size | x.data_ptr()) % 16:
+    st, sh, sd = x.stride()
+    if sd == 1 and not ((st | sh) * x.element_size() | x.data_ptr()) % 16:
         return x
     return x.clone(memory_format=torch.contiguous_format)
+
+
+def _codes(k_cache, v_cache) -> tuple:
+    """(k, v, is_fp8, block and head strides) as the C entry points take a cache's codes."""
+    kb, kh = k_cache.stride()[:2]
+    vb, vh = v_cache.stride()[:2]
+    return k_cache.data_ptr(), v_cache.data_ptr(), int(k_cache.dtype is not torch.int8), kb, kh, vb, vh
 
 
 def store_block_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -203,15 +216,15 @@ def store_block_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.T
         raise ValueError(f"key and value must be fp32, fp16 or bf16 alike, got {key.dtype} and {value.dtype}")
     t = key.shape[0]
     _int32("slot_mapping", slot_mapping, (t,))
-    dev = _on_device("store_block_kvcache", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    dev = _device_index("store_block_kvcache", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     if t == 0:
         return
     key, value = _aligned_rows(key), _aligned_rows(value)
-    _launch(dev, "fdms_store_block_kvcache", key.data_ptr(), value.data_ptr(), nat.dtype_code(key.dtype),
-            key.stride(0), key.stride(1), value.stride(0), value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(),
-            int(k_cache.dtype != torch.int8), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
-            v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), slot_mapping.data_ptr(), t,
-            nb, bs, h, d)
+    kst, ksh, _ = key.stride()
+    vst, vsh, _ = value.stride()
+    _launch(dev, "fdms_store_block_kvcache", key.data_ptr(), value.data_ptr(), nat.dtype_code(key.dtype), kst, ksh,
+            vst, vsh, *_codes(k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0),
+            slot_mapping.data_ptr(), t, nb, bs, h, d)
 
 
 def gather_block_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -224,15 +237,13 @@ def gather_block_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: 
         raise ValueError(f"gather_block_kvcache returns fp32, fp16 or bf16, not {dtype}")
     t = slot_mapping.numel()
     _int32("slot_mapping", slot_mapping, (t,))
-    dev = _on_device("gather_block_kvcache", k_cache, v_cache, k_scale, v_scale, slot_mapping)
-    k = torch.empty((t, h, d), device=dev, dtype=dtype)
-    v = torch.empty((t, h, d), device=dev, dtype=dtype)
+    dev = _device_index("gather_block_kvcache", k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    k = slot_mapping.new_empty((t, h, d), dtype=dtype)
+    v = slot_mapping.new_empty((t, h, d), dtype=dtype)
     if t:
-        _launch(dev, "fdms_gather_block_kvcache", k_cache.data_ptr(), v_cache.data_ptr(),
-                int(k_cache.dtype != torch.int8), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
-                v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0),
-                slot_mapping.data_ptr(), t, nb, bs, h, d, k.data_ptr(), v.data_ptr(), nat.dtype_code(dtype),
-                k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        _launch(dev, "fdms_gather_block_kvcache", *_codes(k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
+                k_scale.stride(0), slot_mapping.data_ptr(), t, nb, bs, h, d, k.data_ptr(), v.data_ptr(),
+                nat.dtype_code(dtype), h * d, d, h * d, d)
     return k, v
 
 
@@ -309,24 +320,24 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if max_context < 0:
         raise ValueError(f"max_context must not be negative, got {max_context}")
     if out is None:
-        out = torch.empty((t, hq, d), device=q.device, dtype=q.dtype)
+        out = q.new_empty((t, hq, d))
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
             (out.stride(0) | out.stride(1)) % 4 or out.data_ptr() % 8:
         raise ValueError("out must have q's shape and type, a contiguous head_dim and 8-byte aligned rows")
-    dev = _on_device("block_attention", q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out,
-                     *(() if cu_seqlens is None else (cu_seqlens,)))
+    dev = _device_index("block_attention", q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, out,
+                        *(() if cu_seqlens is None else (cu_seqlens,)))
     if t == 0:
         return out
     q = _aligned_rows(q)
     few_rows, few_splits, few_share, tile_splits = block_attention_plan(n, h, hq // h, t, max_seqlen, max_context)
     splits = max(few_splits, tile_splits)
     # the splits' partials, the call's own: nothing is shared between streams or captured graphs
-    ws = torch.empty(t * hq * (splits * (d + 2) + 1), device=dev, dtype=torch.float32) if splits > 1 else None
-    _launch(dev, "fdms_block_attention", q.data_ptr(), nat.dtype_code(q.dtype), q.stride(0), q.stride(1), t,
-            k_cache.data_ptr(), v_cache.data_ptr(), int(k_cache.dtype != torch.int8), k_cache.stride(0),
-            k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), k_scale.data_ptr(), v_scale.data_ptr(),
-            k_scale.stride(0), block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(),
-            nat.ptr(cu_seqlens), out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(ws), n, h, hq // h, d, nb, bs,
-            max_seqlen, few_rows, few_splits, few_share, tile_splits,
-            d ** -0.5 if scale is None else float(scale))
+    ws = k_scale.new_empty(t * hq * (splits * (d + 2) + 1)) if splits > 1 else None
+    qst, qsh, _ = q.stride()
+    ost, osh, _ = out.stride()
+    _launch(dev, "fdms_block_attention", q.data_ptr(), nat.dtype_code(q.dtype), qst, qsh, t,
+            *_codes(k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0),
+            block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), nat.ptr(cu_seqlens),
+            out.data_ptr(), ost, osh, nat.ptr(ws), n, h, hq // h, d, nb, bs, max_seqlen, few_rows, few_splits,
+            few_share, tile_splits, d ** -0.5 if scale is None else float(scale))
     return out

@@ -654,8 +654,8 @@ int fdms_store_block_kvcache(const void* key, const void* value, int dtype, int6
                              const int32_t* slot_mapping, int num_tokens, int num_blocks, int block_size,
                              int num_kv_heads, int head_dim, void* stream);
 
-/* Dense rows out_k / out_v [num_tokens, heads, D] (fp32, fp16 or bf16; even
- * strides) = code * scale at slot_mapping[t], any order; a slot outside the
+/* Dense rows out_k / out_v [num_tokens, heads, D] (fp32, fp16 or bf16; 16-byte
+ * aligned, strides multiples of 8) = code * scale at slot_mapping[t], any order; a slot outside the
  * cache gives zeros. */
 int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_fp8, int64_t kc_b, int64_t kc_h,
                               int64_t vc_b, int64_t vc_h, const float* k_scale, const float* v_scale, int64_t sc_b,
