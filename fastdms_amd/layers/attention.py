@@ -4,7 +4,10 @@ Prefill: dense causal attention over the whole prompt (HIP MFMA kernel
 ``fdms_prefill_attention``; the reference uses flash_attn_varlen_func).
 Decode with compact KV: per-layer slice of the [layers, batch, kv_heads]
 metadata, optional unfused append, then ``compact_decode_attention``.
-The dense paged decode path of the reference is not part of this build.
+Without compact KV, with a block KV cache attached (engine.block_kv): the
+reference's dense path (attention.py:75-100) over 8-bit blocks -- the rows are
+stored, prompts that begin in the step attend to themselves, everything else to
+its blocks.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ from torch import nn
 
 from .. import _native as nat
 from ..utils.context import get_context
+from .block_kv import block_attention, store_block_kvcache
 from .compact_attention import (compact_decode_attention, compact_decode_attention_paged,
                                 fused_decode_attention_planned,
                                 fused_dms_rope_store_compact_decode_attention, store_compact_kvcache)
@@ -65,15 +69,23 @@ class Attention(nn.Module):
         self.compact_k_cache = self.compact_v_cache = torch.tensor([])
         # per-kv-head FP8 scales of this layer's arenas ([Hkv] fp32 views) or None
         self.compact_k_scale = self.compact_v_scale = None
+        # (k_cache, v_cache, k_scale, v_scale) of this layer's dense 8-bit blocks, or None
+        self.block_kv_cache = None
         self.layer_id = -1
 
     def forward(self, q, k, v, *, compact_append_stored: bool = False, compact_q_rope: bool = False,
                 positions: torch.Tensor | None = None, cos_sin_cache: torch.Tensor | None = None, out=None):
         ctx = get_context()
+        if self.block_kv_cache is not None and not ctx.compact_kv_enabled and ctx.slot_mapping is not None:
+            store_block_kvcache(k, v, *self.block_kv_cache, ctx.slot_mapping)
+            if ctx.block_tables is not None:  # earlier rows are among the keys
+                return block_attention(q, *self.block_kv_cache, ctx.block_tables, ctx.context_lens,
+                                       cu_seqlens=ctx.cu_seqlens_q, max_seqlen=ctx.max_seqlen_q,
+                                       max_context=ctx.max_seqlen_k, scale=self.scale, out=out)
         if ctx.is_prefill:
             return prefill_attention(q, k, v, ctx.cu_seqlens_q, ctx.max_seqlen_q, self.scale, out=out)
         if not ctx.compact_kv_enabled:
-            raise RuntimeError("dense paged decode is not part of this build; enable compact KV")
+            raise RuntimeError("decode needs compact KV or a block KV cache with the step's slots and tables")
         base, bt, live, slot = self._layer_metadata(ctx)
         if slot is not None and not compact_append_stored:
             store_compact_kvcache(k, v, self.compact_k_cache, self.compact_v_cache, slot,
