@@ -43,9 +43,11 @@ struct BlockAttnArgs {
   int64_t bt_b;
   const int32_t* context;
   const int32_t* cu;  // nullptr: one query row per sequence
-  float* part_o;    // [split][row of q][head][D], unnormalised
-  float* part_ml;   // [split][row of q][head][2]: maximum, sum
-  int* part_used;   // [row of q][head]: splits that hold a part of it
+  // Parts of a row that several splits share: [split][...][head][D] unnormalised
+  // and [split][...][head][2], its maximum and sum.  Of the kernel for few rows
+  // by (sequence, query), of the one for many by row of q.
+  float *few_o, *few_ml, *part_o, *part_ml;
+  int* part_used;   // [row of q][head]: splits of the second kernel that hold a part of it (0 or 1: none)
   int width, num_blocks, shift, num_seqs, num_kv_heads, group, total_rows;
   int few_rows;     // sequences of at most so many rows are block_attn_kernel's, longer ones the tile kernel's
   int q_f16;
@@ -71,9 +73,13 @@ __device__ __forceinline__ int splits_used(int groups, int splits, int share) {
   return min(splits, max(1, (groups + share - 1) / share));
 }
 
-// Where a split's part of (row t of q, head) lies, in rows of D (part_o) or 2 (part_ml).
+// Where a split's part of (row t of q, head) lies, in rows of D (part_o) or 2
+// (part_ml), and that of query i of sequence b in few_o and few_ml.
 __device__ __forceinline__ int64_t part_row(const BlockAttnArgs& a, int split, int t, int head) {
   return ((int64_t)split * a.total_rows + t) * (a.num_kv_heads * a.group) + head;
+}
+__device__ __forceinline__ int64_t few_row(const BlockAttnArgs& a, int split, int b, int i, int head) {
+  return (((int64_t)split * a.num_seqs + b) * a.few_rows + i) * (a.num_kv_heads * a.group) + head;
 }
 
 __device__ __forceinline__ void store_out4(void* out, int64_t at, f32x4_t v, int f16) {
@@ -345,14 +351,14 @@ __global__ __launch_bounds__(256, (kFewWaves<D, MT>)) void block_attn_kernel(con
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees no key: zeros
       store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
     } else {
-      const int64_t at = part_row(a, split, t, head);
-      *(f32x4_t*)(a.part_o + at * D + d) = v;
+      const int64_t at = few_row(a, split, b, r / a.group, head);
+      *(f32x4_t*)(a.few_o + at * D + d) = v;
       if (d == 0) {
-        a.part_ml[2 * at] = top;
-        a.part_ml[2 * at + 1] = sum;
+        a.few_ml[2 * at] = top;
+        a.few_ml[2 * at + 1] = sum;
       }
     }
-    if (a.part_used && split == 0 && d == 0) a.part_used[part_row(a, 0, t, head)] = used;
+    if (a.part_used && split == 0 && d == 0) a.part_used[part_row(a, 0, t, head)] = 0;
   }
 }
 
@@ -761,59 +767,70 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void block_attn_tile_kernel(con
   }
 }
 
-// Joins the splits of the rows that used several: D / 4 lanes hold a split's
-// part.  Few rows of many splits (a decode step) get a workgroup each, which
-// takes 1024 / D splits at a time and meets in LDS, the parts' loads not waiting
-// for the maxima that weigh them; many rows of few splits (SIDE 1) D / 4 lanes
-// each, one split after another.
-template <int D, int SIDE>
-__global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArgs a, int splits) {
-  constexpr int LPR = D / 4, ROWS = 256 / (LPR * SIDE);
-  static_assert(SIDE == 1 || ROWS == 1, "a row per workgroup, or D / 4 lanes a row");
+// Joins the parts of the first kernel's rows, a workgroup per (sequence, query,
+// head): D / 4 lanes hold a split's part, 1024 / D splits at a time, and meet in
+// LDS.  The parts' loads do not wait for the maxima that weigh them.
+template <int D>
+__global__ __launch_bounds__(256) void block_attn_join_few_kernel(const BlockAttnArgs a, int splits, int share) {
+  constexpr int LPR = D / 4, SIDE = 256 / LPR;
   __shared__ f32x4_t s_v[SIDE][LPR];
   __shared__ float s_f[kMaxSplits];
-  const int heads = a.num_kv_heads * a.group, tid = threadIdx.x;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + (SIDE == 1 ? tid / LPR : 0);
-  const int t = (int)(row / heads), head = (int)(row % heads);
+  const unsigned heads = a.num_kv_heads * a.group;
+  const int head = blockIdx.x % heads, i = (blockIdx.x / heads) % a.few_rows, b = blockIdx.x / heads / a.few_rows;
+  const SeqSpan sp = seq_span(a, b);
+  if (i >= sp.n || sp.n > a.few_rows) return;
+  const int used = splits_used((sp.ctx + kGroupKeys - 1) / kGroupKeys, splits, share);
+  if (used == 1) return;
+  const int tid = threadIdx.x, lane = tid & 63, side = tid / LPR, d = (tid % LPR) * 4;
+  const f32x4_t none = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t row = few_row(a, 0, b, i, head), step = few_row(a, 1, 0, 0, 0);
+  f32x4_t p0 = none, p1 = none;
+  if (side < used) p0 = *(const f32x4_t*)(a.few_o + (row + side * step) * D + d);
+  if (side + SIDE < used) p1 = *(const f32x4_t*)(a.few_o + (row + (side + SIDE) * step) * D + d);
+  float top = kNegInf, sum = 0.0f;
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, a.few_ml[2 * (row + s * step)]);  // every wave by itself
+  top = wave_max(top);
+  const float base = top == kNegInf ? 0.0f : top;
+  for (int s = lane; s < used; s += 64) {
+    const float f = __builtin_amdgcn_exp2f(a.few_ml[2 * (row + s * step)] - base);
+    sum += a.few_ml[2 * (row + s * step) + 1] * f;
+    if (tid < 64) s_f[s] = f;
+  }
+  sum = wave_sum(sum);
+  __syncthreads();
+  f32x4_t v = none;
+  if (side < used) v = p0 * s_f[side];
+  if (side + SIDE < used) v += p1 * s_f[side + SIDE];
+  for (int s = side + 2 * SIDE; s < used; s += SIDE) v += *(const f32x4_t*)(a.few_o + (row + s * step) * D + d) * s_f[s];
+  s_v[side][tid % LPR] = v;
+  __syncthreads();
+  if (tid >= LPR) return;
+  for (int k = 1; k < SIDE; ++k) v += s_v[k][tid];
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  store_out4(a.out, (int64_t)(sp.q0 + i) * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
+}
+
+// Joins the parts of the second kernel's rows: many rows of few splits, D / 4
+// lanes a row, one split after another.
+template <int D>
+__global__ __launch_bounds__(256) void block_attn_join_kernel(const BlockAttnArgs a, int splits) {
+  constexpr int LPR = D / 4, ROWS = 256 / LPR;
+  const int heads = a.num_kv_heads * a.group;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
+  const int t = (int)(row / heads), head = (int)(row % heads), d = (threadIdx.x % LPR) * 4;
   if (t >= a.total_rows) return;
   if (a.cu && (t < a.cu[0] || t >= a.cu[a.num_seqs])) return;  // no sequence's row
   const int used = min(a.part_used[row], splits);
   if (used <= 1) return;
-  const int lane = tid & 63, side = SIDE == 1 ? 0 : tid / LPR, d = (tid % LPR) * 4;
-  const f32x4_t none = {0.0f, 0.0f, 0.0f, 0.0f};
   const int64_t step = (int64_t)a.total_rows * heads;
-  f32x4_t v = none;
   float top = kNegInf, sum = 0.0f;
-  if constexpr (SIDE == 1) {
-    for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * (row + s * step)]);
-    const float base = top == kNegInf ? 0.0f : top;
-    for (int s = 0; s < used; ++s) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (row + s * step)] - base);
-      sum += a.part_ml[2 * (row + s * step) + 1] * f;
-      v += *(const f32x4_t*)(a.part_o + (row + s * step) * D + d) * f;
-    }
-  } else {
-    f32x4_t p0 = none, p1 = none;
-    if (side < used) p0 = *(const f32x4_t*)(a.part_o + (row + side * step) * D + d);
-    if (side + SIDE < used) p1 = *(const f32x4_t*)(a.part_o + (row + (side + SIDE) * step) * D + d);
-    for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_ml[2 * (row + s * step)]);  // every wave by itself
-    top = wave_max(top);
-    const float base = top == kNegInf ? 0.0f : top;
-    for (int s = lane; s < used; s += 64) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (row + s * step)] - base);
-      sum += a.part_ml[2 * (row + s * step) + 1] * f;
-      if (tid < 64) s_f[s] = f;
-    }
-    sum = wave_sum(sum);
-    __syncthreads();
-    if (side < used) v = p0 * s_f[side];
-    if (side + SIDE < used) v += p1 * s_f[side + SIDE];
-    for (int s = side + 2 * SIDE; s < used; s += SIDE)
-      v += *(const f32x4_t*)(a.part_o + (row + s * step) * D + d) * s_f[s];
-    s_v[side][tid % LPR] = v;
-    __syncthreads();
-    if (tid >= LPR) return;
-    for (int k = 1; k < SIDE; ++k) v += s_v[k][tid];
+  for (int s = 0; s < used; ++s) top = fmaxf(top, a.part_ml[2 * (row + s * step)]);
+  const float base = top == kNegInf ? 0.0f : top;
+  f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < used; ++s) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (row + s * step)] - base);
+    sum += a.part_ml[2 * (row + s * step) + 1] * f;
+    v += *(const f32x4_t*)(a.part_o + (row + s * step) * D + d) * f;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   store_out4(a.out, (int64_t)t * a.os_t + (int64_t)head * a.os_h + d, v * inv, a.q_f16);
@@ -827,24 +844,27 @@ template <int D, bool FP8>
 static int launch_block_attn(BlockAttnArgs a, int max_seqlen, int few_splits, int few_share, int tile_splits,
                              hipStream_t st) {
   const int64_t pairs = (int64_t)a.num_seqs * a.num_kv_heads, max_rows = (int64_t)max_seqlen * a.group;
+  const int64_t heads = (int64_t)a.num_kv_heads * a.group;
   if (few_splits) {
     const dim3 grid((unsigned)(pairs * few_splits));
     if (a.few_rows * a.group <= 16) block_attn_kernel<D, FP8, 1><<<grid, 256, 0, st>>>(a, few_splits, few_share);
     else block_attn_kernel<D, FP8, 2><<<grid, 256, 0, st>>>(a, few_splits, few_share);
     FDMS_LAUNCH_CHECK();
+    if (few_splits > 1) {
+      const dim3 rows((unsigned)(a.num_seqs * a.few_rows * heads));
+      block_attn_join_few_kernel<D><<<rows, 256, 0, st>>>(a, few_splits, few_share);
+      FDMS_LAUNCH_CHECK();
+    }
   }
   if (tile_splits) {
     const dim3 grid((unsigned)(pairs * tile_splits), (unsigned)((max_rows - 1) / kTileRows + 1));
     block_attn_tile_kernel<D, FP8><<<grid, 64 * kTileWaves, 0, st>>>(a, tile_splits);
     FDMS_LAUNCH_CHECK();
-  }
-  const int splits = few_splits > tile_splits ? few_splits : tile_splits;
-  if (splits > 1) {
-    const unsigned rows = (unsigned)a.total_rows * a.num_kv_heads * a.group;
-    constexpr int kSide = 1024 / D, kPer = 256 / (D / 4);
-    if (rows <= 2048) block_attn_join_kernel<D, kSide><<<dim3(rows), 256, 0, st>>>(a, splits);
-    else block_attn_join_kernel<D, 1><<<dim3((rows - 1) / kPer + 1), 256, 0, st>>>(a, splits);
-    FDMS_LAUNCH_CHECK();
+    if (tile_splits > 1) {
+      constexpr int kPer = 256 / (D / 4);
+      block_attn_join_kernel<D><<<dim3((unsigned)((a.total_rows * heads - 1) / kPer + 1)), 256, 0, st>>>(a, tile_splits);
+      FDMS_LAUNCH_CHECK();
+    }
   }
   return 0;
 }
@@ -872,9 +892,10 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
       os_h % 4 || kc_b % 16 || kc_h % 16 || vc_b % 16 || vc_h % 16)
     return (int)hipErrorInvalidValue;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads, max_rows = (int64_t)max_seqlen * group_size;
-  const int64_t rows = (int64_t)total_rows * num_kv_heads * group_size;
+  const int64_t heads = (int64_t)num_kv_heads * group_size, rows = total_rows * heads;
   if (pairs * splits > 0x7FFFFFFF || (max_rows - 1) / kTileRows + 1 > 65535 || max_rows > 0x7FFFFFFF ||
-      rows > 0x7FFFFFFF)
+      rows > 0x7FFFFFFF ||
+      heads * num_seqs * few_rows > 0x7FFFFFFF)
     return (int)hipErrorInvalidValue;
   if (total_rows == 0) return 0;
   BlockAttnArgs a;
@@ -885,9 +906,14 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   a.k_scale = k_scale, a.v_scale = v_scale, a.sc_b = sc_b;
   a.tables = block_tables, a.bt_b = bt_b, a.width = width;
   a.context = context_lens, a.cu = cu_seqlens;
-  a.part_o = workspace;
-  a.part_ml = workspace + splits * rows * head_dim;
-  a.part_used = splits > 1 ? (int*)(a.part_ml + splits * rows * 2) : nullptr;
+  // (a count of 1 writes no parts)
+  const int64_t few_parts = few_splits > 1 ? few_splits * heads * num_seqs * few_rows : 0;
+  const int64_t tile_parts = tile_splits > 1 ? tile_splits * rows : 0;
+  a.few_o = workspace;
+  a.part_o = a.few_o + few_parts * head_dim;
+  a.few_ml = a.part_o + tile_parts * head_dim;
+  a.part_ml = a.few_ml + few_parts * 2;
+  a.part_used = tile_splits > 1 ? (int*)(a.part_ml + tile_parts * 2) : nullptr;
   a.num_blocks = num_blocks, a.shift = __builtin_ctz(block_size), a.num_seqs = num_seqs;
   a.num_kv_heads = num_kv_heads, a.group = group_size, a.total_rows = total_rows;
   a.few_rows = few_rows, a.q_f16 = q_dtype == kF16, a.scale = scale;

@@ -259,23 +259,32 @@ def block_attention_plan(seqs: int, heads: int, group: int, rows: int, max_seqle
     be of both kinds, and the first then takes those of at most 16.  Splits:
     the first kernel cuts every context into pieces of few_share 64-key groups,
     as many as give three workgroups per CU if all were the longest, between 4
-    and 32; the second takes those, each of at least 512 keys, that take the
-    least rounds x keys of the 512 workgroups (two per CU) the chip holds, over
-    the tiles that ``rows`` can make."""
+    and 32 (more where that would make over 256 pieces of a context, or over 8192
+    in all); the second those, each of at least 512 keys, for which the least
+    time is expected: keys per split times the turns that the tiles' workgroups
+    take at 512 at a time (between whole turns, as equal ones need, and the
+    even share that unequal ones approach), and what a part more to write and
+    join costs (777 queries over 30 000 tokens, 32 / 8 heads of 128, 1 to 5
+    parts: 659, 504, 547, 528, 454 us; a chunk of 1 000 among 15 decoding
+    sequences: 138, 130, 128, 140, 145)."""
     pairs = seqs * heads
     if max_seqlen * group <= 32:
         few_rows = max_seqlen
     else:
         few_rows = 16 // group if seqs > 1 else 0
     groups = -(-max_context // 64)
-    share = min(32, max(4, -(-groups * pairs // 768)))
-    share = max(share, -(-groups // 256))
+    share = max(min(32, max(4, -(-groups * pairs // 768))), -(-groups // 256), -(-groups * pairs // 8192))
     few = max(1, -(-groups // share)) if few_rows else 0
     if few_rows >= max_seqlen:
         return few_rows, few, share, 0
-    tiles = heads * (rows * group // 128 + seqs)
+    tiles = heads * -(-rows * group // 128)
     most = max(1, min(-(-max_context // 512), 16)) if tiles < 1024 else 1
-    return few_rows, few, share, min(range(1, most + 1), key=lambda n: (-(-tiles * n // 512) + 0.1) / n + 0.01 * n)
+
+    def cost(n: int) -> float:
+        turns = tiles * n / 512
+        return (0.5 * -(-tiles * n // 512) + 0.5 * (turns + 0.5)) / n + 1000 / max(max_context, 1) * n
+
+    return few_rows, few, share, min(range(1, most + 1), key=cost)
 
 
 def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -330,9 +339,11 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return out
     q = _aligned_rows(q)
     few_rows, few_splits, few_share, tile_splits = block_attention_plan(n, h, hq // h, t, max_seqlen, max_context)
-    splits = max(few_splits, tile_splits)
-    # the splits' partials, the call's own: nothing is shared between streams or captured graphs
-    ws = k_scale.new_empty(t * hq * (splits * (d + 2) + 1)) if splits > 1 else None
+    # the splits' parts, the call's own: nothing is shared between streams or captured graphs
+    room = few_splits * n * few_rows * hq * (d + 2) if few_splits > 1 else 0
+    if tile_splits > 1:
+        room += t * hq * (tile_splits * (d + 2) + 1)
+    ws = k_scale.new_empty(room) if room else None
     qst, qsh, _ = q.stride()
     ost, osh, _ = out.stride()
     _launch(dev, "fdms_block_attention", q.data_ptr(), nat.dtype_code(q.dtype), qst, qsh, t,

@@ -676,9 +676,10 @@ int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_f
  * query rows (few_rows * group_size <= 32) run on the kernel for few rows with
  * their keys in parts of about few_share groups of 64, at most few_splits, longer ones on the one for many with
  * up to tile_splits (both at most 256); a count of 0 leaves a launch out and is refused where a
- * sequence may need it.  With S the larger count above 1 the workspace holds
- * S * total_rows * heads * group_size * (D + 2) + total_rows * heads *
- * group_size floats (16-byte aligned) that no other call may use meanwhile. */
+ * sequence may need it.  With H = heads * group_size the workspace
+ * holds few_splits * num_seqs * few_rows * H * (D + 2) floats if few_splits > 1
+ * and tile_splits * total_rows * H * (D + 2) floats plus total_rows * H int32 if
+ * tile_splits > 1 (16-byte aligned), which no other call may use meanwhile. */
 int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, int64_t qs_h, int total_rows,
                          const void* k_cache, const void* v_cache, int is_fp8, int64_t kc_b, int64_t kc_h,
                          int64_t vc_b, int64_t vc_h, const float* k_scale, const float* v_scale, int64_t sc_b,
