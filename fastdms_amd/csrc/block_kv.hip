@@ -42,6 +42,7 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
   __shared__ int s_cu[kTabSeqs + 1];
   __shared__ int s_first[kTabSeqs];
   __shared__ int64_t s_wave[2][kTabThreads / kWave];
+  __shared__ int s_bad[kTabThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bs = 1 << shift;
   const int held_free = *count;
@@ -66,12 +67,15 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
     bsum += blk[j];
   }
   const int64_t tinc = wave_scan_i64(tsum), binc = wave_scan_i64(bsum);
+  const int narrow = __any(bad & kTabNarrow) ? kTabNarrow : 0, invalid = __any(bad & kTabInvalid) ? kTabInvalid : 0;
   if (lane == kWave - 1) {
     s_wave[0][wave] = tinc;
     s_wave[1][wave] = binc;
+    s_bad[wave] = narrow | invalid;
   }
   __syncthreads();
   int64_t tbase = tinc - tsum, bbase = binc - bsum, ttotal = 0, btotal = 0;
+  int status = 0;
   for (int w = 0; w < kTabThreads / kWave; ++w) {
     if (w < wave) {
       tbase += s_wave[0][w];
@@ -79,9 +83,10 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
     }
     ttotal += s_wave[0][w];
     btotal += s_wave[1][w];
+    status |= s_bad[w];
   }
-  if (ttotal > num_tokens) bad |= kTabTokensShort;
-  if (btotal > held_free) bad |= kTabNoBlocks;
+  if (ttotal > num_tokens) status |= kTabTokensShort;
+  if (btotal > held_free) status |= kTabNoBlocks;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int b = tid * 4 + j;
@@ -93,9 +98,7 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
     bbase += blk[j];
   }
   if (tid == 0) s_cu[num_seqs] = (int)ttotal;
-  // the flags of all threads (the call is also the barrier behind s_cu)
-  int status = 0;
-  for (int bit = 1; bit <= kTabInvalid; bit <<= 1) status |= __syncthreads_or(bad & bit) ? bit : 0;
+  __syncthreads();
 
   if (blockIdx.x == 0) {
     for (int b = tid; b <= num_seqs; b += kTabThreads) {

@@ -156,8 +156,8 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
         raise ValueError(f"num_tokens must be between 0 and {_INT_MAX}, got {num_tokens}")
     dev = _device_index("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count)
     if out is None:
-        slots, cu, ctx, count, status = cached_lens.new_empty(num_tokens + 2 * n + 3).split(
-            (num_tokens, n + 1, n, 1, 1))
+        slots, cu, ctx, count, status = torch.split_with_sizes(
+            cached_lens.new_empty(num_tokens + 2 * n + 3), (num_tokens, n + 1, n, 1, 1))
         out = BlockTables(slots, cached_lens.new_empty(num_tokens, dtype=torch.int64), cu, ctx, count, status)
     else:
         for what, size in (("slot_mapping", num_tokens), ("cu_seqlens", n + 1), ("context_lens", n),
