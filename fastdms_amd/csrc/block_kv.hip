@@ -16,7 +16,10 @@ namespace fdms {
 //
 // One launch: every workgroup sums the (at most 4096) lengths itself -- 32 KB
 // that sit in the L2 -- and then maps its own tokens by a binary search of cu
-// in LDS.  A second launch for the map would cost more than the repeated sums.
+// in LDS.  A second launch for the map would cost more than the repeated sums:
+// a kernel node of a graph takes 2.4 us here, and this one, a chain of loads
+// (count and lengths, then a table or stack entry) around two barriers, 5.4 us
+// for 256 decoding sequences and 6.7 for 48 prompts of 218 000 tokens.
 constexpr int kTabThreads = 1024;
 constexpr int kTabSeqs = 4 * kTabThreads;
 constexpr int kTabTokens = 2 * kTabThreads;  // tokens mapped per workgroup
@@ -148,8 +151,15 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
 // in registers between their amax and their codes, so each is read once.  When
 // the run raises the block's scale, the rows before it are encoded again.
 //
-// Bound by HBM: 4 bytes read per value pair and 2 written; a prompt's blocks
-// are independent, so the grid covers them all at once.
+// Bound by HBM: 4 bytes read per K and V value pair and 2 written; a prompt's
+// blocks are independent, so the grid covers them all at once.  What counted:
+// every row's load issued before the first is looked at (a row at a time behind
+// its own bounds test took 131 us where all at once take 90: 26 000 rows of 8
+// heads of 128 in blocks of 256), then the heads, and K and V, of the same tokens
+// in neighbouring workgroups, which read whole rows of the projection (72 -> 58:
+// one head's rows alone lie 12 KB apart, on few memory channels), and codes
+// without clamps for waves of finite values; 53 us now, 3.0 TB/s.  17 000 rows of
+// 8 x 64 in blocks of 16: 31 -> 14 us, 3.7 TB/s.
 // N row elements as loaded (two to a register where they are halves), and as fp32.
 template <typename T, int N>
 struct Raw {
@@ -411,7 +421,8 @@ __global__ __launch_bounds__(64 * WAVES) void store_block_kernel(
 // the first is looked at.  K: 16 bytes of a row per lane.  V comes from
 // transposed tiles: a lane holds the 16 tokens of two channels of the tiles that
 // its first and last token lie in -- a run of slots has no others -- and looks up
-// single bytes of any further ones.
+// single bytes of any further ones.  27 000 rows of 8 x 128 39 us (4.3 TB/s),
+// 17 000 of 8 x 64 16 us (3.4); a token at a time 54 and 25.
 // Two values as TO's, to nearest even by the hardware (v_cvt_pk_bf16_f32, v_cvt_pk_f16_f32).
 template <typename TO> struct Pair;
 template <> struct Pair<float> {
