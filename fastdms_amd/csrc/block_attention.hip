@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256, (kFewWaves<D, MT>)) void block_attn_kernel(con
 // Measured: 777 queries over 30 788 tokens, 32 / 8 heads of 128, int8, 457 us with
 // the join (847 TFLOP/s); four prompts of 17 127 tokens, head_dim 64, e4m3fn, 480
 // us (677).  Of the first case's cycles, at the 1.8 GHz that the clock falls to,
-// the matrix cores are busy 46 %, the vector unit 66 % and LDS 46 %: products and
+// the matrix cores are busy 43 %, the vector unit 62 % and LDS 43 %: products and
 // vector work share a wave's issue, and no part dominates (with the scale factors,
 // the conversions, the exponentials or the maxima left out it takes 442, 386, 425,
 // 438 us).  Steps on the way, first / second case: products, conversion, softmax,
