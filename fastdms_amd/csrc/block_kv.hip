@@ -145,21 +145,26 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
 }
 
 // ------------------------------------------------------------------ store
-// Rows t0 .. t0 + n - 1 with consecutive slots of one block are a run; the
-// workgroup whose tokens hold a run's first row stores the whole run, one wave
-// per 16-row tile of the block, for one kv head and K or V.  The new rows stay
-// in registers between their amax and their codes, so each is read once.  When
-// the run raises the block's scale, the rows before it are encoded again.
+// Rows t .. t + n - 1 with consecutive slots of one block are a run, and it is
+// stored, for one kv head and K or V, by the workgroup whose tokens hold its
+// first row: a run inside one 16-row tile by a wave, so that a decode step's rows,
+// a block each, go side by side; a longer one by the four waves, a tile at a
+// time.  The rows' amax gives the block's scale before they are encoded; a wave
+// keeps its last tile's rows in registers between the two and reads the others
+// again, from the caches.  When the run raises the block's scale, the rows before
+// it are encoded again.
 //
-// Bound by HBM: 4 bytes read per K and V value pair and 2 written; a prompt's
-// blocks are independent, so the grid covers them all at once.  What counted:
-// every row's load issued before the first is looked at (a row at a time behind
-// its own bounds test took 131 us where all at once take 90: 26 000 rows of 8
-// heads of 128 in blocks of 256), then the heads, and K and V, of the same tokens
-// in neighbouring workgroups, which read whole rows of the projection (72 -> 58:
-// one head's rows alone lie 12 KB apart, on few memory channels), and codes
-// without clamps for waves of finite values; 53 us now, 3.0 TB/s.  17 000 rows of
-// 8 x 64 in blocks of 16: 31 -> 14 us, 3.7 TB/s.
+// Bound by HBM: 4 bytes read per K and V value pair and 2 written.  What counted
+// for prompts: every row's load issued before the first is looked at (a row at a
+// time behind its own bounds test took 131 us where all at once take 90: 26 000
+// rows of 8 heads of 128 in blocks of 256), the heads, and K and V, of the same
+// tokens in neighbouring workgroups, which read whole rows of the projection (72
+// -> 58: one head's rows alone lie 12 KB apart, on few memory channels), and codes
+// without clamps for waves of finite values.  And for decode steps, whose runs
+// have one row: a wave per run instead of a workgroup the size of a block, with
+// 600 rows in blocks of 256 16.5 us instead of 688, 33 rows 4.7 instead of 11.7.
+// The four waves cost prompts something (the 26 000 rows 64 us, where a wave per
+// tile of the block took 53), but no call needs waves that have no row.
 // N row elements as loaded (two to a register where they are halves), and as fp32.
 template <typename T, int N>
 struct Raw {
@@ -187,21 +192,6 @@ struct Raw {
     return ld<T>((const T*)&e);
   }
 };
-
-// Max over the workgroup (WAVES waves); every thread calls it.
-template <int WAVES>
-__device__ __forceinline__ float team_max(float v, float* s_red) {
-  v = wave_max(v);
-  if constexpr (WAVES > 1) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = s_red[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) v = fmaxf(v, s_red[w]);
-  }
-  return v;
-}
 
 // Codes of four values x, times inv = 1 / scale.  A wave all of whose values are
 // finite needs neither clamp nor NaN test: |x| / scale is at most the largest
@@ -234,184 +224,272 @@ __device__ __forceinline__ float joined_scale(float amax, int off, float old) {
   return off > 0 ? fmaxf(old, need) : need;
 }
 
-template <typename T, int D, bool FP8, int WAVES>
-__device__ __forceinline__ void store_run_k(const T* __restrict__ x, int64_t xs_t, uint8_t* block, float* scale,
-                                            int off, int n, float* s_red) {
-  constexpr int LPR = D / 8, RPP = kWave / LPR, PASS = kTile / RPP;
-  const int lane = lane_id(), tile0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kTile;
-  const int row0 = tile0 + lane / LPR, d0 = (lane % LPR) * 8;
-  const float old = *scale;
-  Raw<T, 8> v[PASS] = {};
-  float amax = 0.0f, odd = 0.0f;  // odd: NaN once a value is infinite or NaN
-  if (tile0 < off + n && tile0 + kTile > off) {  // some of the wave's rows are new
-    if (tile0 >= off && tile0 + kTile <= off + n) {  // all of them: one address per lane, the passes at scalar steps
-      const T* p = x + (int64_t)(row0 - off) * xs_t + d0;
+// What a run does to its block: rows off .. off + n - 1 are new.
+struct Run {
+  int off, n;
+  float inv, ratio;  // 1 / scale; the former scale over it
+  bool grown;        // the rows before are encoded again
+};
+
+// A 16-row tile of K in a wave's registers, 8 channels of some rows per lane.
+template <typename T, int D, bool FP8>
+struct TileK {
+  static constexpr int LPR = D / 8, RPP = kWave / LPR, PASS = kTile / RPP;
+  Raw<T, 8> v[PASS];
+  __device__ __forceinline__ static int row() { return lane_id() / LPR; }
+  __device__ __forceinline__ static int channel() { return (lane_id() % LPR) * 8; }
+  __device__ __forceinline__ void load(const T* x, int64_t xs_t, int tile, int off, int n) {
+    const int r0 = tile * kTile - off;
+    if (r0 >= 0 && r0 + kTile <= n) {  // all rows new: one address per lane, the passes at scalar steps
+      const T* p = x + (int64_t)(r0 + row()) * xs_t + channel();
 #pragma unroll
       for (int i = 0; i < PASS; ++i) v[i].load(p + i * RPP * xs_t);
-    } else {  // rows past the run are its first or last again
+    } else {  // in place of rows outside the run its first or last again
 #pragma unroll
-      for (int i = 0; i < PASS; ++i) v[i].load(x + (int64_t)min(max(row0 + i * RPP - off, 0), n - 1) * xs_t + d0);
+      for (int i = 0; i < PASS; ++i)
+        v[i].load(x + (int64_t)min(max(r0 + row() + i * RPP, 0), n - 1) * xs_t + channel());
     }
+  }
+  // largest magnitude; odd: NaN once a value is infinite or NaN
+  __device__ __forceinline__ void look(float* amax, float* odd) const {
 #pragma unroll
     for (int i = 0; i < PASS; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        amax = fmaxf(amax, fabsf(v[i][j]));
-        odd = __builtin_fmaf(v[i][j], 0.0f, odd);
+        *amax = fmaxf(*amax, fabsf(v[i][j]));
+        *odd = __builtin_fmaf(v[i][j], 0.0f, *odd);
       }
   }
-  const float s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old), inv = 1.0f / s;
-  u32x2_t c[PASS];
-  if (!__any(odd != odd)) {
+  __device__ __forceinline__ void store(uint8_t* block, int tile, const Run& run, bool finite) const {
+    u32x2_t c[PASS];
+    if (finite) {
 #pragma unroll
-    for (int i = 0; i < PASS; ++i)
+      for (int i = 0; i < PASS; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        c[i][j] = encode4_finite<FP8>(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3], inv);
-  } else {
+        for (int j = 0; j < 2; ++j)
+          c[i][j] = encode4_finite<FP8>(v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3], run.inv);
+    } else {
 #pragma unroll
-    for (int i = 0; i < PASS; ++i)
+      for (int i = 0; i < PASS; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        c[i][j] = encode4<FP8>(nan_to_zero(v[i][4 * j]) * inv, nan_to_zero(v[i][4 * j + 1]) * inv,
-                               nan_to_zero(v[i][4 * j + 2]) * inv, nan_to_zero(v[i][4 * j + 3]) * inv);
+        for (int j = 0; j < 2; ++j)
+          c[i][j] = encode4<FP8>(nan_to_zero(v[i][4 * j]) * run.inv, nan_to_zero(v[i][4 * j + 1]) * run.inv,
+                                 nan_to_zero(v[i][4 * j + 2]) * run.inv, nan_to_zero(v[i][4 * j + 3]) * run.inv);
+    }
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int r = tile * kTile + row() + i * RPP;
+      if (r >= run.off && r < run.off + run.n) *(u32x2_t*)(block + r * D + channel()) = c[i];
+    }
+    if (run.grown && tile * kTile < run.off) again(block, tile, run);
   }
-  const bool grown = off > 0 && s > old;
-  const float ratio = old * inv;
+  // the tile's rows before the run
+  __device__ __forceinline__ static void again(uint8_t* block, int tile, const Run& run) {
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int r = row0 + i * RPP;
-    u32x2_t* dst = (u32x2_t*)(block + r * D + d0);
-    if (r >= off && r < off + n) {
-      *dst = c[i];
-    } else if (grown && r < off) {
-      u32x2_t was = *dst;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) was[j] = encode4_again<FP8>(was[j], ratio);
-      *dst = was;
+    for (int i = 0; i < PASS; ++i) {
+      const int r = tile * kTile + row() + i * RPP;
+      u32x2_t* p = (u32x2_t*)(block + r * D + channel());
+      if (r < run.off) {
+        u32x2_t was = *p;
+        was[0] = encode4_again<FP8>(was[0], run.ratio);
+        was[1] = encode4_again<FP8>(was[1], run.ratio);
+        *p = was;
+      }
     }
   }
-  if (threadIdx.x == 0) *scale = s;
-}
+};
 
-// V: a lane holds two channels of 16 (D = 128) or 8 (D = 64) tokens of its
-// wave's tile, the bytes it stores.
-template <typename T, int D, bool FP8, int WAVES>
-__device__ __forceinline__ void store_run_v(const T* __restrict__ x, int64_t xs_t, uint8_t* block, float* scale,
-                                            int off, int n, float* s_red) {
-  constexpr int LPR = D / 2, TOK = kTile * LPR / kWave, WORDS = TOK / 4;
+// And of V: two channels of 16 (D = 128) or 8 (D = 64) tokens per lane, the bytes it stores.
+template <typename T, int D, bool FP8>
+struct TileV {
+  static constexpr int LPR = D / 2, TOK = kTile * LPR / kWave, WORDS = TOK / 4;
   typedef uint32_t words_t __attribute__((ext_vector_type(WORDS)));
-  const int lane = lane_id(), tile0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kTile;
-  const int d0 = (lane % LPR) * 2, t0 = (lane / LPR) * TOK, row0 = tile0 + t0;
-  const float old = *scale;
-  Raw<T, 2> v[TOK] = {};
-  float amax = 0.0f, odd = 0.0f;
-  if (tile0 < off + n && tile0 + kTile > off) {
-    if (tile0 >= off && tile0 + kTile <= off + n) {
-      const T* p = x + (int64_t)(row0 - off) * xs_t + d0;
+  static constexpr int STEP = kTile / (4 * WORDS);  // words_t's from a channel's tokens to the next one's
+  Raw<T, 2> v[TOK];
+  __device__ __forceinline__ static int row() { return lane_id() / LPR * TOK; }
+  __device__ __forceinline__ static int channel() { return (lane_id() % LPR) * 2; }
+  __device__ __forceinline__ static words_t* place(uint8_t* block, int tile) {
+    return (words_t*)(block + tile * (kTile * D) + channel() * kTile + row());
+  }
+  __device__ __forceinline__ void load(const T* x, int64_t xs_t, int tile, int off, int n) {
+    const int r0 = tile * kTile - off;
+    if (r0 >= 0 && r0 + kTile <= n) {
+      const T* p = x + (int64_t)(r0 + row()) * xs_t + channel();
 #pragma unroll
       for (int j = 0; j < TOK; ++j) v[j].load(p + j * xs_t);
     } else {
 #pragma unroll
-      for (int j = 0; j < TOK; ++j) v[j].load(x + (int64_t)min(max(row0 + j - off, 0), n - 1) * xs_t + d0);
+      for (int j = 0; j < TOK; ++j) v[j].load(x + (int64_t)min(max(r0 + row() + j, 0), n - 1) * xs_t + channel());
     }
+  }
+  __device__ __forceinline__ void look(float* amax, float* odd) const {
 #pragma unroll
     for (int j = 0; j < TOK; ++j) {
-      amax = fmaxf(amax, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
-      odd = __builtin_fmaf(v[j][0], 0.0f, odd);
-      odd = __builtin_fmaf(v[j][1], 0.0f, odd);
+      *amax = fmaxf(*amax, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
+      *odd = __builtin_fmaf(v[j][0], 0.0f, *odd);
+      *odd = __builtin_fmaf(v[j][1], 0.0f, *odd);
     }
   }
-  const float s = joined_scale<FP8>(team_max<WAVES>(amax, s_red), off, old), inv = 1.0f / s;
-  const bool grown = off > 0 && s > old;
-  if (threadIdx.x == 0) *scale = s;
-  if (!(row0 < off + n && row0 + TOK > off) && !(grown && row0 < off)) return;  // nothing of the lane's changes
-  words_t code[2];
-  if (!__any(odd != odd)) {
+  __device__ __forceinline__ void store(uint8_t* block, int tile, const Run& run, bool finite) const {
+    words_t code[2];
+    if (finite) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w)
-        code[c][w] = encode4_finite<FP8>(v[4 * w][c], v[4 * w + 1][c], v[4 * w + 2][c], v[4 * w + 3][c], inv);
-  } else {
+        for (int w = 0; w < WORDS; ++w)
+          code[c][w] = encode4_finite<FP8>(v[4 * w][c], v[4 * w + 1][c], v[4 * w + 2][c], v[4 * w + 3][c], run.inv);
+    } else {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w)
-        code[c][w] = encode4<FP8>(nan_to_zero(v[4 * w][c]) * inv, nan_to_zero(v[4 * w + 1][c]) * inv,
-                                  nan_to_zero(v[4 * w + 2][c]) * inv, nan_to_zero(v[4 * w + 3][c]) * inv);
-  }
-  words_t* dst = (words_t*)(block + tile0 * D + d0 * kTile + t0);
-  constexpr int STEP = kTile / (4 * WORDS);  // words_t's from a channel's tokens to the next one's
-  if (!(row0 >= off && row0 + TOK <= off + n)) {
-    // bytes of the rows before (encoded again if the scale grew) and of those behind
-    const float ratio = old * inv;
+        for (int w = 0; w < WORDS; ++w)
+          code[c][w] = encode4<FP8>(nan_to_zero(v[4 * w][c]) * run.inv, nan_to_zero(v[4 * w + 1][c]) * run.inv,
+                                    nan_to_zero(v[4 * w + 2][c]) * run.inv, nan_to_zero(v[4 * w + 3][c]) * run.inv);
+    }
+    words_t* p = place(block, tile);
+    const int r0 = tile * kTile + row();
+    if (!(r0 >= run.off && r0 + TOK <= run.off + run.n)) {
+      // bytes of the rows before (encoded again if the scale grew) and of those behind
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const words_t was = dst[c * STEP];
+      for (int c = 0; c < 2; ++c) {
+        const words_t was = p[c * STEP];
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        const uint32_t again = grown ? encode4_again<FP8>(was[w], ratio) : was[w];
-        uint32_t mixed = 0;
+        for (int w = 0; w < WORDS; ++w) {
+          const uint32_t old = run.grown ? encode4_again<FP8>(was[w], run.ratio) : was[w];
+          uint32_t mixed = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = row0 + 4 * w + j;
-          const uint32_t from = r < off ? again : (r < off + n ? code[c][w] : was[w]);
-          mixed |= from & (0xFFu << (8 * j));
+          for (int j = 0; j < 4; ++j) {
+            const int r = r0 + 4 * w + j;
+            const uint32_t from = r < run.off ? old : (r < run.off + run.n ? code[c][w] : was[w]);
+            mixed |= from & (0xFFu << (8 * j));
+          }
+          code[c][w] = mixed;
         }
-        code[c][w] = mixed;
       }
     }
+    p[0] = code[0];
+    p[STEP] = code[1];
   }
-  dst[0] = code[0];
-  dst[STEP] = code[1];
+  __device__ __forceinline__ static void again(uint8_t* block, int tile, const Run& run) {  // all rows before the run
+    words_t* p = place(block, tile);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      words_t was = p[c * STEP];
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) was[w] = encode4_again<FP8>(was[w], run.ratio);
+      p[c * STEP] = was;
+    }
+  }
+};
+
+constexpr int kStoreWaves = 4;
+
+// A run by one wave (its rows lie in one tile) or by the workgroup.
+template <typename TILE, bool TEAM, bool FP8, typename T>
+__device__ __forceinline__ void store_run(const T* x, int64_t xs_t, uint8_t* block, float* scale, int off, int n,
+                                          float* s_red) {
+  const int first = off / kTile, last = (off + n - 1) / kTile, step = TEAM ? kStoreWaves : 1;
+  const int wave = TEAM ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const float old = *scale;
+  TILE tile;
+  float amax = 0.0f, odd = 0.0f;
+  int held = -1;  // the tile in registers
+  for (int i = first + wave; i <= last; i += step) {
+    tile.load(x, xs_t, i, off, n);
+    tile.look(&amax, &odd);
+    held = i;
+  }
+  amax = wave_max(amax);
+  if constexpr (TEAM) {
+    __syncthreads();  // the last run's maxima have been read
+    if (lane_id() == 0) s_red[wave] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  }
+  const float s = joined_scale<FP8>(amax, off, old);
+  Run run;
+  run.off = off, run.n = n, run.inv = 1.0f / s, run.ratio = old * run.inv, run.grown = off > 0 && s > old;
+  const bool finite = !__any(odd != odd);
+  for (int i = held; i >= first; i -= step) {
+    if (i != held) tile.load(x, xs_t, i, off, n);
+    tile.store(block, i, run, finite);
+  }
+  if (run.grown)
+    for (int i = wave; i < first; i += step) TILE::again(block, i, run);
+  if (TEAM ? threadIdx.x == 0 : lane_id() == 0) *scale = s;
 }
 
-template <typename T, int D, bool FP8, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void store_block_kernel(
+template <typename T, int D, bool FP8>
+__global__ __launch_bounds__(64 * kStoreWaves) void store_block_kernel(
     const T* __restrict__ k, int64_t ks_t, int64_t ks_h, const T* __restrict__ v, int64_t vs_t, int64_t vs_h,
     uint8_t* kc, int64_t kc_b, int64_t kc_h, uint8_t* vc, int64_t vc_b, int64_t vc_h, float* k_scale,
-    float* v_scale, int64_t sc_b, const int32_t* __restrict__ slots,
-    int num_tokens, int num_blocks, int num_heads, int per_group) {
-  constexpr int BS = kTile * WAVES;
-  __shared__ float s_red[WAVES];
+    float* v_scale, int64_t sc_b, const int32_t* __restrict__ slots, int num_tokens, int num_blocks, int shift,
+    int num_heads, int chunk) {
+  __shared__ float s_red[kStoreWaves];
+  __shared__ int s_long[kWave][2];  // runs for the workgroup: first token, rows
+  __shared__ int s_count;
   // heads, and K and V, run fastest: workgroups that run together read whole rows of the projection
   const unsigned heads2 = 2 * num_heads, part = blockIdx.x % heads2;
-  const int h = part % num_heads, lane = lane_id();
+  const int h = part % num_heads, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool is_v = part >= (unsigned)num_heads;
-  int64_t t = (int64_t)(blockIdx.x / heads2) * per_group;
-  const int64_t end = min(t + per_group, (int64_t)num_tokens);
-  while (t < end) {
-    const int slot = slots[t];
-    const int blk = slot / BS, off = slot & (BS - 1);
-    if (slot < 0 || blk >= num_blocks) {
-      ++t;
-      continue;
-    }
-    const bool first = off == 0 || t == 0 || slots[t - 1] != slot - 1;
-    int n = 0;  // rows of the run: the leading lanes whose slots follow on
-    constexpr int LOOKS = (BS + kWave - 1) / kWave;
+  const T* x = is_v ? v + h * vs_h : k + h * ks_h;
+  const int64_t xs_t = is_v ? vs_t : ks_t, c_b = is_v ? vc_b : kc_b;
+  uint8_t* base = is_v ? vc + h * vc_h : kc + h * kc_h;
+  float* scale = (is_v ? v_scale : k_scale) + h;
+  const int bs = 1 << shift;
+  const int64_t t0 = (int64_t)(blockIdx.x / heads2) * chunk;
+  // lane i looks at token t0 + i: does a run begin there?
+  const int64_t mine = t0 + lane;
+  const bool here = lane < chunk && mine < num_tokens;
+  const int slot_l = here ? slots[mine] : -1, before = here && mine > 0 ? slots[mine - 1] : -1;
+  const bool leads = slot_l >= 0 && (slot_l >> shift) < num_blocks &&
+                     ((slot_l & (bs - 1)) == 0 || mine == 0 || before != slot_l - 1);
+  uint64_t leaders = __ballot(leads);
+  if (leaders == 0) return;  // the same in all waves
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  for (int turn = 0; leaders; ++turn) {
+    const int i = __builtin_ctzll(leaders);
+    leaders &= leaders - 1;
+    if (turn % kStoreWaves != wave) continue;
+    const int slot = __builtin_amdgcn_readlane(slot_l, i), off = slot & (bs - 1);
+    const int64_t t = t0 + i;
+    int n = 0;  // the leading rows whose slots follow on, all looked up at once
+    constexpr int LOOKS = (1 << kMaxBlockLog2) / kWave;
     int seen[LOOKS];
 #pragma unroll
-    for (int k = 0; k < LOOKS; ++k) seen[k] = slots[min(t + k * kWave + lane, (int64_t)num_tokens - 1)];
+    for (int j = 0; j < LOOKS; ++j)
+      seen[j] = j == 0 || j * kWave < bs ? slots[min(t + j * kWave + lane, (int64_t)num_tokens - 1)] : -1;
     bool whole = true;
 #pragma unroll
-    for (int k = 0; k < LOOKS; ++k) {
-      const int i = k * kWave + lane;
-      const uint64_t m = ~__ballot(off + i < BS && t + i < num_tokens && seen[k] == slot + i);
-      const int run = m ? __builtin_ctzll(m) : kWave;
-      n += whole ? run : 0;
-      whole = whole && run == kWave;
+    for (int j = 0; j < LOOKS; ++j) {
+      const int at = j * kWave + lane;
+      const uint64_t m = ~__ballot(off + at < bs && t + at < num_tokens && seen[j] == slot + at);
+      const int rows = m ? __builtin_ctzll(m) : kWave;
+      n += whole ? rows : 0;
+      whole = whole && rows == kWave;
     }
-    if (first) {
+    if (off / kTile == (off + n - 1) / kTile) {
+      const int64_t blk = slot >> shift;
       if (is_v)
-        store_run_v<T, D, FP8, WAVES>(v + t * vs_t + h * vs_h, vs_t, vc + blk * vc_b + h * vc_h,
-                                      v_scale + blk * sc_b + h, off, n, s_red);
+        store_run<TileV<T, D, FP8>, false, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
       else
-        store_run_k<T, D, FP8, WAVES>(k + t * ks_t + h * ks_h, ks_t, kc + blk * kc_b + h * kc_h,
-                                      k_scale + blk * sc_b + h, off, n, s_red);
+        store_run<TileK<T, D, FP8>, false, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
+    } else if (lane == 0) {
+      const int at = atomicAdd(&s_count, 1);  // (whatever their order, the runs are independent)
+      s_long[at][0] = i;
+      s_long[at][1] = n;
     }
-    t += n;
+  }
+  __syncthreads();
+  for (int j = 0; j < s_count; ++j) {
+    const int i = __builtin_amdgcn_readfirstlane(s_long[j][0]), n = __builtin_amdgcn_readfirstlane(s_long[j][1]);
+    const int slot = __builtin_amdgcn_readlane(slot_l, i), off = slot & (bs - 1);
+    const int64_t t = t0 + i, blk = slot >> shift;
+    if (is_v)
+      store_run<TileV<T, D, FP8>, true, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
+    else
+      store_run<TileK<T, D, FP8>, true, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
   }
 }
 
@@ -565,28 +643,6 @@ FDMS_EXPORT int fdms_block_tables(const int32_t* cached_lens, const int32_t* new
   return 0;
 }
 
-template <typename T, int D, bool FP8>
-static int launch_store(int block_size, dim3 grid, hipStream_t st, const void* k, int64_t ks_t, int64_t ks_h,
-                        const void* v, int64_t vs_t, int64_t vs_h, void* kc, int64_t kc_b, int64_t kc_h, void* vc,
-                        int64_t vc_b, int64_t vc_h, float* k_scale, float* v_scale, int64_t sc_b,
-                        const int32_t* slots, int num_tokens, int num_blocks, int num_heads, int per_group) {
-#define FDMS_STORE(W)                                                                                             \
-  store_block_kernel<T, D, FP8, W><<<grid, 64 * W, 0, st>>>((const T*)k, ks_t, ks_h, (const T*)v, vs_t, vs_h,     \
-                                                            (uint8_t*)kc, kc_b, kc_h, (uint8_t*)vc, vc_b, vc_h,   \
-                                                            k_scale, v_scale, sc_b, slots, num_tokens, num_blocks, \
-                                                            num_heads, per_group)
-  switch (block_size / kTile) {
-    case 1: FDMS_STORE(1); break;
-    case 2: FDMS_STORE(2); break;
-    case 4: FDMS_STORE(4); break;
-    case 8: FDMS_STORE(8); break;
-    default: FDMS_STORE(16); break;
-  }
-#undef FDMS_STORE
-  FDMS_LAUNCH_CHECK();
-  return 0;
-}
-
 FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int dtype, int64_t ks_t, int64_t ks_h,
                                          int64_t vs_t, int64_t vs_h, void* k_cache, void* v_cache, int is_fp8,
                                          int64_t kc_b, int64_t kc_h, int64_t vc_b, int64_t vc_h, float* k_scale,
@@ -594,7 +650,7 @@ FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int
                                          int num_blocks, int block_size, int num_kv_heads, int head_dim,
                                          void* stream) {
   if (dtype < kF32 || dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 ||
-      ((int64_t)num_tokens / 16 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
+      ((int64_t)num_tokens / 64 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
     return (int)hipErrorInvalidValue;
   if (!block_cache_ok(k_cache, kc_b, kc_h, v_cache, vc_b, vc_h, num_blocks, block_size, head_dim))
     return (int)hipErrorInvalidValue;
@@ -602,19 +658,29 @@ FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int
   if (!fdms_aligned16(key, value) || ks_t * size % 16 || ks_h * size % 16 || vs_t * size % 16 || vs_h * size % 16)
     return (int)hipErrorInvalidValue;
   if (num_tokens == 0) return 0;
-  // A workgroup looks for runs in as many tokens as a block holds: a prompt's
-  // workgroups then find one or two each.  A step of few tokens, whose rows
-  // lie in a block each, gets a workgroup per token, so none stores several.
-  const int per_group = num_tokens <= 512 ? 1 : block_size;
-  const dim3 grid(((num_tokens - 1) / per_group + 1) * 2u * num_kv_heads);
-#define FDMS_ARGS                                                                                                 \
-  block_size, grid, (hipStream_t)stream, key, ks_t, ks_h, value, vs_t, vs_h, k_cache, kc_b, kc_h, v_cache, vc_b,  \
-      vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, num_blocks, num_kv_heads, per_group
+  // Tokens whose runs a workgroup stores, at most one for each of its lanes: few
+  // where they may be a decode step's, with a run each (a wave then stores one;
+  // 33 rows and their read-back 26 us, with 64 tokens a workgroup 31), many where
+  // most lie inside a prompt's runs and begin none (17 000 rows of 8 heads of 64
+  // and their read-back 31 us, with 4 tokens a workgroup 94).
+  const int chunk = num_tokens <= 2048 ? kStoreWaves : kWave;
+  const dim3 grid(((num_tokens - 1) / chunk + 1) * 2u * num_kv_heads);
+#define FDMS_STORE(TT, D, F)                                                                                       \
+  store_block_kernel<TT, D, F><<<grid, 64 * kStoreWaves, 0, (hipStream_t)stream>>>(                                \
+      (const TT*)key, ks_t, ks_h, (const TT*)value, vs_t, vs_h, (uint8_t*)k_cache, kc_b, kc_h, (uint8_t*)v_cache,  \
+      vc_b, vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, num_blocks, __builtin_ctz(block_size),         \
+      num_kv_heads, chunk)
   FDMS_DISPATCH_FLOAT(dtype, T, {
-    if (head_dim == 64) return is_fp8 ? launch_store<T, 64, true>(FDMS_ARGS) : launch_store<T, 64, false>(FDMS_ARGS);
-    return is_fp8 ? launch_store<T, 128, true>(FDMS_ARGS) : launch_store<T, 128, false>(FDMS_ARGS);
+    if (head_dim == 64) {
+      if (is_fp8) FDMS_STORE(T, 64, true);
+      else FDMS_STORE(T, 64, false);
+    } else {
+      if (is_fp8) FDMS_STORE(T, 128, true);
+      else FDMS_STORE(T, 128, false);
+    }
   });
-#undef FDMS_ARGS
+#undef FDMS_STORE
+  FDMS_LAUNCH_CHECK();
   return 0;
 }
 
@@ -625,7 +691,7 @@ FDMS_EXPORT int fdms_gather_block_kvcache(const void* k_cache, const void* v_cac
                                           int head_dim, void* out_k, void* out_v, int out_dtype, int64_t ok_t,
                                           int64_t ok_h, int64_t ov_t, int64_t ov_h, void* stream) {
   if (out_dtype < kF32 || out_dtype > kBF16 || num_tokens < 0 || num_kv_heads < 1 ||
-      ((int64_t)num_tokens / 16 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
+      ((int64_t)num_tokens / 64 + 512) * 2 * num_kv_heads > 0x7FFFFFFF)  // workgroups of the grid
     return (int)hipErrorInvalidValue;
   if (!block_cache_ok(k_cache, kc_b, kc_h, v_cache, vc_b, vc_h, num_blocks, block_size, head_dim))
     return (int)hipErrorInvalidValue;

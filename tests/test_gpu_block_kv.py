@@ -185,6 +185,27 @@ def test_store_and_gather_equal_the_definition(dtype, d, bs, lens):
 
 
 @pytest.mark.parametrize("dtype", [torch.int8, FP8])
+@pytest.mark.parametrize("bs", [16, 128, 256])
+@pytest.mark.parametrize("lens", [
+    ([17 * i % 300 for i in range(200)], [1] * 200),                               # many runs of a row
+    ([3] * 12 + [0, 250], [2] * 12 + [2000, 700]),                                 # short runs beside long ones
+    ([17 * i % 90 for i in range(61)], [1] * 30 + [0] + [40 + i for i in range(30)]),
+])
+@pytest.mark.parametrize("pad", [0, 2500])
+def test_store_of_many_runs(dtype, bs, lens, pad):
+    """Decode rows, short and long runs in one call, with and without padding (calls under and over 2048 rows)."""
+    kv, h, d = _kv(), 2, 64
+    nb, earlier, slots, _ = _store_case(bs, *lens)
+    cache = _garbage_cache(nb, h, bs, d, dtype)
+    want = ref.Cache(cache)
+    for step, (at, grow) in enumerate(((earlier, 0.5), (slots + [-1] * pad, 1.0))):
+        k, v = (_rows(len(at), h, d, torch.bfloat16, 10 * step + i, grow) for i in range(2))
+        kv.store_block_kvcache(k, v, *cache, _ints(at))
+        want.store(k, v, at)
+    _same_cache(cache, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, FP8])
 @pytest.mark.parametrize("rows", [torch.float32, torch.float16, torch.bfloat16])
 def test_store_takes_strided_and_unaligned_rows_and_any_float(dtype, rows):
     kv, h, d, bs = _kv(), 2, 64, 32
