@@ -626,14 +626,32 @@ static bool block_cache_ok(const void* kc, int64_t kc_b, int64_t kc_h, const voi
          kc_h % 16 == 0 && vc_b % 16 == 0 && vc_h % 16 == 0;
 }
 
+// Whether [a, a + n) and [b, b + m) of elements of the given sizes meet.
+inline bool meet(const void* a, int64_t n, int size_a, const void* b, int64_t m, int size_b) {
+  const char *p = (const char*)a, *q = (const char*)b;
+  return n > 0 && m > 0 && p < q + m * size_b && q < p + n * size_a;
+}
+
 FDMS_EXPORT int fdms_block_tables(const int32_t* cached_lens, const int32_t* new_lens, int num_seqs,
                                   int32_t* block_tables, int64_t bt_b, int width, const int32_t* free_blocks,
                                   int num_free_blocks, const int32_t* free_count, int block_size, int num_tokens,
                                   int32_t* slot_mapping, int64_t* positions, int32_t* cu_seqlens,
                                   int32_t* context_lens, int32_t* free_count_out, int32_t* status, void* stream) {
   if (num_seqs < 1 || num_seqs > kTabSeqs || width < 0 || num_free_blocks < 0 || num_tokens < 0 ||
-      block_size < 16 || block_size > 256 || (block_size & (block_size - 1)) || free_count_out == free_count)
+      block_size < 16 || block_size > 256 || (block_size & (block_size - 1)))
     return (int)hipErrorInvalidValue;
+  // workgroups read the inputs while others write the outputs
+  const struct {
+    const void* at;
+    int64_t n;
+    int size;
+  } in[] = {{cached_lens, num_seqs, 4}, {new_lens, num_seqs, 4}, {block_tables, (num_seqs - 1) * bt_b + width, 4},
+            {free_blocks, num_free_blocks, 4}, {free_count, 1, 4}},
+    out[] = {{slot_mapping, num_tokens, 4}, {positions, num_tokens, 8}, {cu_seqlens, num_seqs + 1, 4},
+             {context_lens, num_seqs, 4}, {free_count_out, 1, 4}, {status, 1, 4}};
+  for (const auto& i : in)
+    for (const auto& o : out)
+      if (meet(i.at, i.n, i.size, o.at, o.n, o.size)) return (int)hipErrorInvalidValue;
   const int groups = num_tokens ? (num_tokens - 1) / kTabTokens + 1 : 1;
   block_tables_kernel<<<groups, kTabThreads, 0, (hipStream_t)stream>>>(
       cached_lens, new_lens, num_seqs, block_tables, bt_b, width, free_blocks, num_free_blocks, free_count,

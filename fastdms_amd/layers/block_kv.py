@@ -116,6 +116,20 @@ def _int32(what: str, t: torch.Tensor, shape: tuple) -> None:
         raise ValueError(f"{what} must be a contiguous int32 {list(shape)} tensor, got {t.dtype} {list(t.shape)}")
 
 
+def _overlap(outs, ins) -> bool:
+    """Whether the memory of one of the contiguous ``outs`` meets an input's span."""
+    spans = []
+    for x in ins:
+        if x.numel():
+            size = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+            spans.append((x.data_ptr(), x.data_ptr() + size * x.element_size()))
+    for o in outs:
+        start, end = o.data_ptr(), o.data_ptr() + o.numel() * o.element_size()
+        if any(start < b and a < end for a, b in spans):
+            return True
+    return False
+
+
 def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
                          free_blocks: torch.Tensor, free_count: torch.Tensor, *, block_size: int, num_tokens: int,
                          out: BlockTables | None = None) -> BlockTables:
@@ -136,7 +150,8 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
     popped: the tables stay, every slot is -1, cu_seqlens is 0 and context_lens
     the cached lengths.  ``free_count`` is not changed in place, so a step can
     be prepared again; ``out`` takes an earlier call's tensors (captured steps),
-    whose free_count must be another tensor than the argument."""
+    which share no memory with the arguments: the launch's workgroups read those
+    while others write."""
     n = cached_lens.numel()
     if not 1 <= n <= MAX_SEQS:
         raise ValueError(f"prepare_block_tables takes 1 to {MAX_SEQS} sequences, got {n}")
@@ -154,21 +169,21 @@ def prepare_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, bloc
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
     if not 0 <= num_tokens <= _INT_MAX:
         raise ValueError(f"num_tokens must be between 0 and {_INT_MAX}, got {num_tokens}")
-    dev = _device_index("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count)
-    if out is None:
-        slots, cu, ctx, count, status = torch.split_with_sizes(
-            cached_lens.new_empty(num_tokens + 2 * n + 3), (num_tokens, n + 1, n, 1, 1))
-        out = BlockTables(slots, cached_lens.new_empty(num_tokens, dtype=torch.int64), cu, ctx, count, status)
-    else:
+    if out is not None:
         for what, size in (("slot_mapping", num_tokens), ("cu_seqlens", n + 1), ("context_lens", n),
                            ("free_count", 1), ("status", 1)):
             _int32(f"out.{what}", getattr(out, what), (size,))
         if out.positions.dtype != torch.int64 or out.positions.shape != (num_tokens,) or \
                 not out.positions.is_contiguous():
             raise ValueError(f"out.positions must be a contiguous int64 [{num_tokens}] tensor")
-        _device_index("prepare_block_tables", cached_lens, *out)
-        if out.free_count.data_ptr() == free_count.data_ptr():
-            raise ValueError("out.free_count must be another tensor than free_count")
+        if _overlap(out, (cached_lens, new_lens, block_tables, free_blocks, free_count)):
+            raise ValueError("out's tensors must not share memory with the lengths, tables, free list or count")
+    dev = _device_index("prepare_block_tables", cached_lens, new_lens, block_tables, free_blocks, free_count,
+                        *(() if out is None else out))
+    if out is None:
+        slots, cu, ctx, count, status = torch.split_with_sizes(
+            cached_lens.new_empty(num_tokens + 2 * n + 3), (num_tokens, n + 1, n, 1, 1))
+        out = BlockTables(slots, cached_lens.new_empty(num_tokens, dtype=torch.int64), cu, ctx, count, status)
     _launch(dev, "fdms_block_tables", cached_lens.data_ptr(), new_lens.data_ptr(), n, block_tables.data_ptr(),
             block_tables.stride(0), width, free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(),
             block_size, num_tokens, out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.cu_seqlens.data_ptr(),

@@ -627,8 +627,8 @@ int fdms_fp8_gemm(const void* x, int64_t x_s, const float* x_inv, const void* w,
  * from free_blocks[0 .. *free_count), top first, in sequence order, and
  * written to its row.  Token t < num_tokens gets slot_mapping[t] and
  * positions[t] (-1 and 0 past the last token); cu_seqlens [num_seqs + 1],
- * context_lens = cached + new, *free_count_out = what is left (not the same
- * address as free_count).  *status is 0, or the sum of 1 (too few free
+ * context_lens = cached + new, *free_count_out = what is left.  The outputs
+ * may not share memory with the inputs.  *status is 0, or the sum of 1 (too few free
  * blocks), 2 (a table row too narrow), 4 (num_tokens too small) and 8 (a
  * negative length, a context from 2^31, or a count outside 0 ..
  * num_free_blocks); then the tables are left alone, slots are -1, cu_seqlens

@@ -57,6 +57,40 @@ def test_block_tables_out_must_fit():
         _tables(out=out())
 
 
+def test_block_tables_out_must_not_meet_the_inputs():
+    """Outputs in the inputs' memory (an in-place step) are refused, neighbours in one buffer are not."""
+    def out(**change):
+        a = dict(slot_mapping=torch.zeros(2, dtype=I32), positions=torch.zeros(2, dtype=torch.int64),
+                 cu_seqlens=torch.zeros(3, dtype=I32), context_lens=torch.zeros(2, dtype=I32),
+                 free_count=torch.zeros(1, dtype=I32), status=torch.zeros(1, dtype=I32))
+        a.update(change)
+        return kv.BlockTables(**a)
+    buf = torch.zeros(16, dtype=I32)
+    for argument, mine, field, theirs in (
+            ("cached_lens", buf[:2], "context_lens", buf[:2]), ("new_lens", buf[:2], "context_lens", buf[1:3]),
+            ("cached_lens", buf[2:4], "cu_seqlens", buf[:3]), ("free_count", buf[:1], "free_count", buf[:1]),
+            ("free_count", buf[:1], "status", buf[:1]), ("free_blocks", buf[:5], "slot_mapping", buf[3:5]),
+            ("block_tables", buf[:14].view(2, 7)[:, :4], "context_lens", buf[9:11]),
+            ("free_blocks", buf[:5], "positions", buf[2:6].view(torch.int64))):
+        with pytest.raises(ValueError, match="share memory"):
+            _tables(**{argument: mine}, out=out(**{field: theirs}))
+    with pytest.raises(RuntimeError):  # (the device check, after every other)
+        _tables(cached_lens=buf[:2], new_lens=buf[2:4], out=out(context_lens=buf[4:6], cu_seqlens=buf[6:9]))
+
+
+def test_library_refuses_tables_that_meet():
+    if not _native.LIB_PATH.exists():
+        pytest.skip("library not built")
+    p = [ctypes.c_void_p(i << 12) for i in range(1, 16)]
+
+    def tables(cached=p[0], table=p[2], free=p[3], count=p[4], slots=p[5], cu=p[7], ctx=p[8], status=p[10]):
+        return _native.lib().fdms_block_tables(cached, p[1], 2, table, 5, 4, free, 1, count, 16, 1024, slots, p[6], cu,
+                                               ctx, p[9], status, None)
+    for bad in (dict(ctx=p[0]), dict(ctx=p[1]), dict(cu=p[4]), dict(status=p[4]), dict(status=p[3]),
+                dict(ctx=ctypes.c_void_p(p[2].value + 32)), dict(cached=ctypes.c_void_p(p[5].value + 4092))):
+        assert tables(**bad) == 1, bad
+
+
 @pytest.mark.parametrize("op", ["tables", "store", "gather", "attention"])
 def test_cpu_tensors_are_refused(op):
     c = _cache()
