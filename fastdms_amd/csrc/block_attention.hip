@@ -21,6 +21,7 @@
 // rounding to bf16 (2^-8) stays the error there is.  Row sums stay in fp32, of the
 // unrounded weights in the kernel for few rows and of the rounded ones (which the
 // numerator has) in the one for many.
+#include <cmath>
 #include <type_traits>
 
 #include "fdms_block_kv.h"
@@ -407,7 +408,8 @@ __global__ __launch_bounds__(256, (kFewWaves<D, MT>)) void block_attn_kernel(con
 // before those.
 //
 // The blocks' scales go into the halves: a block's codes times its scale over
-// the largest so far (a power of two no greater than 1 for the store's scales).
+// the largest so far (a power of two no greater than 1 for the store's scales;
+// other ratios are rounded to a half, and the products with them).
 // What falls below a half's range there is 2^-25 of that largest scale, far less
 // than the fp32 sum it joins can hold next to it.  Then one factor holds for all
 // keys of a step, and exp(s - max) is one fma and one v_exp_f32 per score.
@@ -907,7 +909,7 @@ FDMS_EXPORT int fdms_block_attention(const void* q, int q_dtype, int64_t qs_t, i
   if ((q_dtype != kF16 && q_dtype != kBF16) || total_rows < 0 || num_seqs < 1 || num_kv_heads < 1 || group_size < 1 ||
       (head_dim != 64 && head_dim != 128) || max_seqlen < 1 || width < 0 || num_blocks < 1 || block_size < 16 ||
       block_size > 256 || (block_size & (block_size - 1)) ||
-      (cu_seqlens == nullptr && (max_seqlen != 1 || total_rows != num_seqs)))
+      (cu_seqlens == nullptr && (max_seqlen != 1 || total_rows != num_seqs)) || !std::isfinite(scale))
     return (int)hipErrorInvalidValue;
   // every sequence length has its kernel: up to few_rows query rows the one, past them the other
   const int splits = few_splits > tile_splits ? few_splits : tile_splits;

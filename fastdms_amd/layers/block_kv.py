@@ -17,6 +17,7 @@ pack a prompt into the compact layout.
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -316,8 +317,10 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     contexts (default: what a table row can hold); both are host numbers that
     shape the launch.  A query that sees no key gets zeros, rows past
     ``cu_seqlens[-1]`` of ``out`` are left as they are, and keys of a block
-    that is not in the cache are left out.  Scales must not be negative.
-    Default ``scale``: D ** -0.5."""
+    that is not in the cache are left out.  Default ``scale`` (any finite
+    number): D ** -0.5.  The cache's scales must not be negative; those that
+    are not powers of two are taken exactly for the queries of few-row
+    sequences, and else codes times scales are rounded to 2^-10 of themselves."""
     nb, h, bs, d = _check_cache(k_cache, v_cache, k_scale, v_scale)
     if q.ndim != 3 or q.shape[2] != d or q.shape[1] % h or q.shape[1] == 0:
         raise ValueError(f"expected q [rows, a multiple of {h} heads, {d}], got {tuple(q.shape)}")
@@ -343,6 +346,9 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     max_context = width * bs if max_context is None else int(max_context)
     if max_context < 0:
         raise ValueError(f"max_context must not be negative, got {max_context}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
     if out is None:
         out = q.new_empty((t, hq, d))
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or \
@@ -365,5 +371,5 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             *_codes(k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0),
             block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), nat.ptr(cu_seqlens),
             out.data_ptr(), ost, osh, nat.ptr(ws), n, h, hq // h, d, nb, bs, max_seqlen, few_rows, few_splits,
-            few_share, tile_splits, d ** -0.5 if scale is None else float(scale))
+            few_share, tile_splits, scale)
     return out

@@ -671,7 +671,10 @@ int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_f
  * query row per sequence (total_rows = num_seqs, max_seqlen 1).  max_seqlen
  * bounds the query rows of a sequence.  Contexts past what a table row can
  * hold are cut; keys of a block outside the cache are left out; a query that
- * sees no key gets zeros; rows outside cu_seqlens are not written.  q rows
+ * sees no key gets zeros; rows outside cu_seqlens are not written.  scale must
+ * be finite and the cache's scales not negative; those that are not powers of
+ * two are exact on the kernel for few rows, and on the other codes times scales
+ * are rounded to 2^-10 of themselves.  q rows
  * 16-byte, out rows 8-byte aligned.  Sequences of up to few_rows
  * query rows (few_rows * group_size <= 32) run on the kernel for few rows with
  * their keys in parts of about few_share groups of 64, at most few_splits, longer ones on the one for many with

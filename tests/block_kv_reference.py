@@ -92,7 +92,7 @@ def tables(cached, new, table, free, count, bs, num_tokens):
     return (table, slots + [-1] * pad, positions + [0] * pad, cu, [c + n for c, n in zip(cached, new)], count)
 
 
-def attention(q, cache: Cache, table, context, cu, scale=None):
+def attention(q, cache: Cache, table, context, cu, scale=None, codes=0.0):
     """(out, bound) [T, Hq, D] in 64 bits.  The bound is what the kernel's
     roundings can add up to, element by element (half a unit in the last place
     is eps / 2 of the value):
@@ -105,6 +105,11 @@ def attention(q, cache: Cache, table, context, cu, scale=None):
     * codes may be held as halves relative to the largest scale of the
       sequence, and then are off by at most 2^-25 of it: e_s grows by scale *
       2^-25 max sK * sum |q|, the result by 2^-25 max sV;
+    * scales that are not powers of two: a block's scale over the sequence's
+      largest may be rounded to a half and a code's product with it again, each
+      2^-11 of itself.  With ``codes`` = 2^-10 + 2^-22 K's part of that is
+      codes * |scale| * sum |k q| more in e_s, which is then no longer small
+      enough for exp(2 e_s) - 1 = 2 e_s; V's is codes * sum_j p_j |v_j|;
     * the result is rounded once to its type: eps / 2 of itself."""
     t, hq, d = q.shape
     nb, h = cache.scale["k"].shape
@@ -139,9 +144,13 @@ def attention(q, cache: Cache, table, context, cu, scale=None):
                 a = p @ vv[:, j // g].abs()
                 es = float(s.abs().max()) * (d + 8) * 2.0 ** -24
                 es += abs(scale) * 2.0 ** -25 * tops[0][j // g] * float(q[q0 + i, j].abs().sum())
+                shift = 2 * es
+                if codes:
+                    es += codes * abs(scale) * float((kk[:, j // g].abs() @ q[q0 + i, j].abs()).max())
+                    shift = math.expm1(2 * es) + codes
                 top = float(p.max())
                 out[q0 + i, j] = o
-                err = a * (2.0 ** -11 + 2 * es + n * 2.0 ** -24) + top * n * 2.0 ** -25 * float(vv.abs().max())
+                err = a * (2.0 ** -11 + shift + n * 2.0 ** -24) + top * n * 2.0 ** -25 * float(vv.abs().max())
                 err = err + 2.0 ** -25 * tops[1][j // g]
                 bound[q0 + i, j] = err + half * (o.abs() + err)
     return out, bound

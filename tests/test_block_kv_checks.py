@@ -192,6 +192,7 @@ def _attend(**change):
     dict(cu_seqlens=torch.zeros(3, dtype=torch.int64)),
     dict(cu_seqlens=None),
     dict(max_seqlen=0), dict(max_context=-1),
+    dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-float("inf")),
     dict(out=torch.zeros(5, 4, 64)),
     dict(out=torch.zeros(4, 4, 64, dtype=torch.bfloat16)),
     dict(out=torch.zeros(5, 64, 4, dtype=torch.bfloat16).transpose(1, 2)),
@@ -233,12 +234,13 @@ def test_library_refuses_without_launching():
     assert gather(tokens=0) == 0
 
     def attend(q=p[0], dtype=_native.DT_BF16, rows=2, cu=p[7], out=p[8], ws=p[9], seqs=2, h=1, g=4, d=64, nb=4, bs=16,
-               most=1, few=1, splits=1, share=4, tiles=0, os_t=256):
+               most=1, few=1, splits=1, share=4, tiles=0, os_t=256, scale=0.1):
         return lib.fdms_block_attention(q, dtype, 256, 64, rows, p[2], p[3], 0, 1024, 1024, 1024, 1024, p[4], p[5], 1,
                                         p[6], 4, 4, p[10], cu, out, os_t, 64, ws, seqs, h, g, d, nb, bs, most, few,
-                                        splits, share, tiles, 0.1, None)
+                                        splits, share, tiles, scale, None)
     for bad in (dict(q=ctypes.c_void_p(4104)), dict(dtype=_native.DT_F32), dict(rows=-1), dict(out=ctypes.c_void_p(4098)),
                 dict(splits=0), dict(splits=2, ws=None), dict(splits=-1), dict(splits=257), dict(share=0), dict(seqs=0), dict(h=0), dict(g=0), dict(d=96), dict(nb=0),
-                dict(bs=20), dict(most=0), dict(few=-1, tiles=1), dict(few=9), dict(most=2), dict(few=0, splits=0), dict(cu=None, rows=3), dict(cu=None, most=2), dict(os_t=6)):
+                dict(bs=20), dict(most=0), dict(few=-1, tiles=1), dict(few=9), dict(most=2), dict(few=0, splits=0), dict(cu=None, rows=3), dict(cu=None, most=2), dict(os_t=6),
+                dict(scale=float("inf")), dict(scale=float("nan"))):
         assert attend(**bad) == 1, bad
     assert attend(rows=0) == 0

@@ -305,7 +305,7 @@ def _attend_case(bs, h, d, dtype, context, seed=0, spare=2):
 
 
 def _check_attention(cache, table, context, lens, group, dtype=torch.bfloat16, seed=0, scale=None, q=None, pad=0,
-                     max_context=None, mag=1.0):
+                     max_context=None, mag=1.0, codes=0.0):
     kv = _kv()
     nb, h, bs, d = cache[0].shape
     cu = ref.cu_of(lens)
@@ -317,7 +317,7 @@ def _check_attention(cache, table, context, lens, group, dtype=torch.bfloat16, s
     got = kv.block_attention(q, *cache, _ints(table), _ints(context), cu_seqlens=_ints(cu), max_seqlen=max(lens),
                              max_context=max_context, scale=scale, out=out)
     assert got.data_ptr() == out.data_ptr()
-    want, bound = ref.attention(q, ref.Cache(cache), table, context, cu, scale)
+    want, bound = ref.attention(q, ref.Cache(cache), table, context, cu, scale, codes)
     far = (got.cpu().double() - want).abs()[:cu[-1]]
     assert (far <= bound[:cu[-1]]).all(), f"{(far - bound[:cu[-1]]).max()} past the bound, {far.max()} off"
     assert (got[cu[-1]:] == 7.0).all()
@@ -402,6 +402,19 @@ def test_attention_scales_that_differ_widely(n):
     _check_attention(cache, table, [16 * 9], [n], 4)
     cache[2].copy_(torch.exp2(torch.linspace(-30, -3, cache[2].numel(), device=DEV).round()).view_as(cache[2]))
     _check_attention(cache, table, [16 * 9], [n], 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 7, 60])
+def test_attention_scales_that_are_no_powers_of_two(dtype, d, n):
+    """Exact for few rows, rounded to halves relative to the largest for many (the bound's codes)."""
+    context = [16 * 9 + 5, 200]
+    cache, table = _attend_case(32, 2, d, dtype, context)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    for x in cache[2:]:
+        x *= 1 + torch.rand(x.shape, generator=g, device=DEV)
+    _check_attention(cache, table, context, [n, n], 4, mag=0.25, codes=2.0 ** -10 + 2.0 ** -22 if n > 8 else 0.0)
 
 
 @pytest.mark.parametrize("n", [4, 36])
