@@ -18,7 +18,11 @@ from ..utils.context import reset_context, set_context
 class BlockKVManager:
     """``num_blocks`` blocks per layer and up to ``max_seqs`` sequences of up to
     ``max_model_len`` tokens.  One table serves all layers: a block id is the
-    same rows of each layer's cache."""
+    same rows of each layer's cache.
+
+    For eager steps: the host plans each from its counts, and ``free_count`` is
+    another tensor after a step or a release.  A captured step calls
+    ``prepare_block_tables`` on tensors of its own."""
 
     def __init__(self, *, num_layers: int, num_kv_heads: int, head_dim: int, num_blocks: int, max_seqs: int,
                  max_model_len: int, block_size: int = 256, dtype: torch.dtype = torch.int8, device="cuda"):
