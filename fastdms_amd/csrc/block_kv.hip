@@ -162,9 +162,7 @@ __global__ __launch_bounds__(kTabThreads) void block_tables_kernel(
 // -> 58: one head's rows alone lie 12 KB apart, on few memory channels), and codes
 // without clamps for waves of finite values.  And for decode steps, whose runs
 // have one row: a wave per run instead of a workgroup the size of a block, with
-// 600 rows in blocks of 256 16.5 us instead of 688, 33 rows 4.7 instead of 11.7.
-// The four waves cost prompts something (the 26 000 rows 64 us, where a wave per
-// tile of the block took 53), but no call needs waves that have no row.
+// 600 rows in blocks of 256 16.1 us instead of 688, 33 rows 4.8 instead of 11.7.
 // N row elements as loaded (two to a register where they are halves), and as fp32.
 template <typename T, int N>
 struct Raw {
@@ -424,9 +422,9 @@ __global__ __launch_bounds__(64 * kStoreWaves) void store_block_kernel(
     const T* __restrict__ k, int64_t ks_t, int64_t ks_h, const T* __restrict__ v, int64_t vs_t, int64_t vs_h,
     uint8_t* kc, int64_t kc_b, int64_t kc_h, uint8_t* vc, int64_t vc_b, int64_t vc_h, float* k_scale,
     float* v_scale, int64_t sc_b, const int32_t* __restrict__ slots, int num_tokens, int num_blocks, int shift,
-    int num_heads, int chunk) {
+    int num_heads, int tokens) {
   __shared__ float s_red[kStoreWaves];
-  __shared__ int s_long[kWave][2];  // runs for the workgroup: first token, rows
+  __shared__ int s_long[kStoreWaves * kWave][3];  // runs for the workgroup: first token, its slot, rows
   __shared__ int s_count;
   // heads, and K and V, run fastest: workgroups that run together read whole rows of the projection
   const unsigned heads2 = 2 * num_heads, part = blockIdx.x % heads2;
@@ -437,21 +435,18 @@ __global__ __launch_bounds__(64 * kStoreWaves) void store_block_kernel(
   uint8_t* base = is_v ? vc + h * vc_h : kc + h * kc_h;
   float* scale = (is_v ? v_scale : k_scale) + h;
   const int bs = 1 << shift;
-  const int64_t t0 = (int64_t)(blockIdx.x / heads2) * chunk;
-  // lane i looks at token t0 + i: does a run begin there?
-  const int64_t mine = t0 + lane;
-  const bool here = lane < chunk && mine < num_tokens;
+  // lane i looks at the wave's token i: does a run begin there?
+  const int64_t t0 = ((int64_t)(blockIdx.x / heads2) * kStoreWaves + wave) * tokens, mine = t0 + lane;
+  const bool here = lane < tokens && mine < num_tokens;
   const int slot_l = here ? slots[mine] : -1, before = here && mine > 0 ? slots[mine - 1] : -1;
   const bool leads = slot_l >= 0 && (slot_l >> shift) < num_blocks &&
                      ((slot_l & (bs - 1)) == 0 || mine == 0 || before != slot_l - 1);
   uint64_t leaders = __ballot(leads);
-  if (leaders == 0) return;  // the same in all waves
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  for (int turn = 0; leaders; ++turn) {
+  while (leaders) {
     const int i = __builtin_ctzll(leaders);
     leaders &= leaders - 1;
-    if (turn % kStoreWaves != wave) continue;
     const int slot = __builtin_amdgcn_readlane(slot_l, i), off = slot & (bs - 1);
     const int64_t t = t0 + i;
     int n = 0;  // the leading rows whose slots follow on, all looked up at once
@@ -477,15 +472,17 @@ __global__ __launch_bounds__(64 * kStoreWaves) void store_block_kernel(
         store_run<TileK<T, D, FP8>, false, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
     } else if (lane == 0) {
       const int at = atomicAdd(&s_count, 1);  // (whatever their order, the runs are independent)
-      s_long[at][0] = i;
-      s_long[at][1] = n;
+      s_long[at][0] = (int)t;
+      s_long[at][1] = slot;
+      s_long[at][2] = n;
     }
   }
   __syncthreads();
   for (int j = 0; j < s_count; ++j) {
-    const int i = __builtin_amdgcn_readfirstlane(s_long[j][0]), n = __builtin_amdgcn_readfirstlane(s_long[j][1]);
-    const int slot = __builtin_amdgcn_readlane(slot_l, i), off = slot & (bs - 1);
-    const int64_t t = t0 + i, blk = slot >> shift;
+    const int64_t t = __builtin_amdgcn_readfirstlane(s_long[j][0]);
+    const int slot = __builtin_amdgcn_readfirstlane(s_long[j][1]), n = __builtin_amdgcn_readfirstlane(s_long[j][2]);
+    const int64_t blk = slot >> shift;
+    const int off = slot & (bs - 1);
     if (is_v)
       store_run<TileV<T, D, FP8>, true, FP8>(x + t * xs_t, xs_t, base + blk * c_b, scale + blk * sc_b, off, n, s_red);
     else
@@ -676,18 +673,20 @@ FDMS_EXPORT int fdms_store_block_kvcache(const void* key, const void* value, int
   if (!fdms_aligned16(key, value) || ks_t * size % 16 || ks_h * size % 16 || vs_t * size % 16 || vs_h * size % 16)
     return (int)hipErrorInvalidValue;
   if (num_tokens == 0) return 0;
-  // Tokens whose runs a workgroup stores, at most one for each of its lanes: few
-  // where they may be a decode step's, with a run each (a wave then stores one;
-  // 33 rows and their read-back 26 us, with 64 tokens a workgroup 31), many where
-  // most lie inside a prompt's runs and begin none (17 000 rows of 8 heads of 64
-  // and their read-back 31 us, with 4 tokens a workgroup 94).
-  const int chunk = num_tokens <= 2048 ? kStoreWaves : kWave;
-  const dim3 grid(((num_tokens - 1) / chunk + 1) * 2u * num_kv_heads);
+  // Tokens whose runs a wave looks for, at most one for each of its lanes: one
+  // where they may be a decode step's, with a run each, then so many that the
+  // grid has the 4096 waves the card holds (8 heads of 128, blocks of 256: 2000
+  // decode rows 45 us and a run of 2000 rows 8.8; with twice the waves 42 and 11.7,
+  // with half 62 and 9.1; with a token a wave 44 and 15), up to a block's or 64 per
+  // workgroup, past which workgroups would have several long runs to store.
+  const int most = block_size <= 64 ? 16 : block_size / 4;
+  const int tokens = (int)std::min<int64_t>(std::max<int64_t>((int64_t)num_tokens * 2 * num_kv_heads / 4096, 1), most);
+  const dim3 grid(((num_tokens - 1) / (tokens * kStoreWaves) + 1) * 2u * num_kv_heads);
 #define FDMS_STORE(TT, D, F)                                                                                       \
   store_block_kernel<TT, D, F><<<grid, 64 * kStoreWaves, 0, (hipStream_t)stream>>>(                                \
       (const TT*)key, ks_t, ks_h, (const TT*)value, vs_t, vs_h, (uint8_t*)k_cache, kc_b, kc_h, (uint8_t*)v_cache,  \
       vc_b, vc_h, k_scale, v_scale, sc_b, slot_mapping, num_tokens, num_blocks, __builtin_ctz(block_size),         \
-      num_kv_heads, chunk)
+      num_kv_heads, tokens)
   FDMS_DISPATCH_FLOAT(dtype, T, {
     if (head_dim == 64) {
       if (is_fp8) FDMS_STORE(T, 64, true);

@@ -191,9 +191,9 @@ def test_store_and_gather_equal_the_definition(dtype, d, bs, lens):
     ([3] * 12 + [0, 250], [2] * 12 + [2000, 700]),                                 # short runs beside long ones
     ([17 * i % 90 for i in range(61)], [1] * 30 + [0] + [40 + i for i in range(30)]),
 ])
-@pytest.mark.parametrize("pad", [0, 2500])
+@pytest.mark.parametrize("pad", [0, 2500, 60000])
 def test_store_of_many_runs(dtype, bs, lens, pad):
-    """Decode rows, short and long runs in one call, with and without padding (calls under and over 2048 rows)."""
+    """Decode rows, short and long runs in one call, with and without padding (a wave looks at 1 to 64 tokens)."""
     kv, h, d = _kv(), 2, 64
     nb, earlier, slots, _ = _store_case(bs, *lens)
     cache = _garbage_cache(nb, h, bs, d, dtype)
