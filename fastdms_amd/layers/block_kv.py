@@ -2,7 +2,7 @@
 
 The cache that keeps every token, beside the compact one that DMS evicts from
 (the reference's dense paged path, attention.py:17-37, 94-100, keeps bf16 rows
-and calls flash-attn).  Blocks of ``block_size`` tokens (a power of two,
+and calls a library for attention).  Blocks of ``block_size`` tokens (a power of two,
 16 .. 256) hold each kv head's rows in 8 bits with one scale per (block, head)
 for K and one for V:
 

@@ -663,8 +663,8 @@ int fdms_gather_block_kvcache(const void* k_cache, const void* v_cache, int is_f
                               int num_kv_heads, int head_dim, void* out_k, void* out_v, int out_dtype, int64_t ok_t,
                               int64_t ok_h, int64_t ov_t, int64_t ov_h, void* stream);
 
-/* Causal GQA attention over the cache (replaces flash_attn_with_kvcache and
- * the paged flash_attn_varlen_func of attention.py:85-100): sequence b has
+/* Causal GQA attention over the cache (replaces the library calls over
+ * the paged cache of attention.py:85-100): sequence b has
  * query rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of q / out [total_rows, heads *
  * group_size, D] (bf16 or fp16), the last of its context_lens[b] keys, which
  * its table row (width entries, stride bt_b) leads to.  cu_seqlens NULL: one
