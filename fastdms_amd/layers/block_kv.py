@@ -230,6 +230,10 @@ def store_block_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.T
                          f"{tuple(value.shape)}")
     if key.dtype not in _FLOATS or value.dtype != key.dtype:
         raise ValueError(f"key and value must be fp32, fp16 or bf16 alike, got {key.dtype} and {value.dtype}")
+    if k_scale.data_ptr() == v_scale.data_ptr() or nb > 1 and 0 in (k_cache.stride(0), v_cache.stride(0),
+                                                                    k_scale.stride(0)) or \
+            h > 1 and 0 in (k_cache.stride(1), v_cache.stride(1)):
+        raise ValueError("K and V, blocks and heads need memory of their own to be stored into")
     t = key.shape[0]
     _int32("slot_mapping", slot_mapping, (t,))
     dev = _device_index("store_block_kvcache", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)

@@ -163,6 +163,16 @@ def test_store_refuses(key, value, slots):
         kv.store_block_kvcache(key, value, *_cache(), slots)
 
 
+def test_store_refuses_memory_that_is_shared():
+    """K and V with one scale tensor, and blocks or heads expanded from one: workgroups would race on them."""
+    k, v, ks, vs = _cache()
+    rows, slots = torch.zeros(2, 2, 64), torch.zeros(2, dtype=I32)
+    for bad in ((k, v, ks, ks), (k[:1].expand(3, -1, -1, -1), v, ks, vs), (k, v[:, :1].expand(-1, 2, -1, -1, -1), ks, vs),
+                (k, v, ks[:1].expand(3, -1), vs[:1].expand(3, -1))):
+        with pytest.raises(ValueError, match="memory of their own"):
+            kv.store_block_kvcache(rows, rows, *bad, slots)
+
+
 def test_gather_refuses_other_types():
     with pytest.raises(ValueError):
         kv.gather_block_kvcache(*_cache(), torch.zeros(3, dtype=I32), dtype=torch.int8)
